@@ -33,6 +33,12 @@ extern "C" {
 #define VK_DEVERR_WAIT_EMPTY 2u  /* a producer gave up waiting for a free stage */
 #define VK_DEVERR_WAIT_ACCUM 4u  /* an epilogue gave up waiting for the tensor-core accumulator */
 #define VK_DEVERR_BOUNDS 8u      /* an index (token, position, cache row) was out of range; access skipped */
+#define VK_DEVERR_PAGES 16u      /* no free cache page was left; the row it was for was not changed */
+
+/* Element types of the entry points that take more than one. */
+#define VK_BF16 0
+#define VK_F16 1
+#define VK_F32 2
 
 /* Library version as major*10000 + minor*100 + patch. */
 int vk_version(void);
@@ -264,6 +270,75 @@ int vk_prefill_plan(const int32_t* lens, int n, int row0, int pos_scale, int64_t
 int vk_scatter_embed(void* x, const int64_t* rows, int64_t n, int64_t x_rows, const void* emb, int64_t token,
                      int d, void* stream);
 
+
+/* ---- several candidates of a chunk: a shared prefix, tails in pages, penalties -----------------------------
+ * No counterpart in the reference, which decodes one row per chunk. */
+
+/* Workspace bytes vk_shared_attention needs (contents do not matter before or after a call). */
+size_t vk_shared_attention_workspace_bytes(int B, int H, int HK, int D, int P, int S, int max_tail);
+
+/* One query token of each of B rows against a prefix shared by a group of rows and a tail of its own:
+ * out[b, h] = sum_j p_j v_j, p = softmax(scale * q[b, h] . k_j) over the prefix_lens[g] positions of prefix g and then
+ * the tail_lens[b] tokens of row b, KV head h / (H / HK), for the rows group_offsets[g] <= b < group_offsets[g + 1].
+ * q [B, H, D] (row stride stride_q elements), out [B, H, D] and the caches in one type (VK_BF16 or VK_F16), D 64 or
+ * 128, HK divides H, 0 < scale < inf.  k_prefix / v_prefix: element (g, p, kvh, d) at g * stride_kb + p * stride_ks +
+ * kvh * D + d, p < S, strides multiples of 8 (one layer of a static cache whose rows are the prefixes).  k_pages /
+ * v_pages: n_pages pages of `page` tokens (a power of two, 8..256), element (page, slot, kvh, d) at page * stride_pp +
+ * (slot * HK + kvh) * D + d; page_table [B, max_pages] i32 (row stride stride_table) names row b's pages.
+ * prefix_lens [P], group_offsets [P + 1] (ascending from 0, at most B), tail_lens [B] i32.  lse [B, H] f32 (log of the sum of
+ * exponentials) or NULL.  A row with nothing to attend gets 0 and lse -inf; rows behind the last group are left as they
+ * were.  What lies behind a prefix's or a tail's length is not used, whatever it holds.  Lengths, offsets and pages out
+ * of range are reported in the device error word (results of those rows are unspecified).  out must not overlap q. */
+int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* k_prefix, const void* v_prefix,
+                        const int32_t* prefix_lens, const int32_t* group_offsets, int P, int S, int64_t stride_kb,
+                        int64_t stride_ks, const void* k_pages, const void* v_pages, int n_pages, int page,
+                        int64_t stride_pp, const int32_t* page_table, int max_pages, int64_t stride_table,
+                        const int32_t* tail_lens, void* out, float* lse, int B, int H, int HK, int D, float scale,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages of a cache.  table [rows, max_pages] i32 names the pages of each row (-1 behind its last), lens [rows] i32 the
+ * tokens of each row, refs [n_pages] i32 how many rows name a page (0: free); page = tokens per page, a power of two,
+ * 8..256.  All but the last page of a row are full and only full pages are shared.  Free pages are given out the lowest
+ * first, in the order of the list.  Row numbers out of range, and all but the first naming of a row that a list names
+ * twice, are skipped and reported (VK_DEVERR_BOUNDS); a row for which no page is left is not changed and reported
+ * (VK_DEVERR_PAGES).  Calls on the same pages follow one another on one stream.
+ * Workspace bytes the three calls below need for n listed rows (contents do not matter). */
+size_t vk_pages_workspace_bytes(int rows, int max_pages, int n_pages, int n);
+
+/* Room for `count` more tokens in each of the rows list[0 .. n) (NULL: all rows, n = rows): lens grows by count, and
+ * token j's place is page_out / slot_out [n, count] i32 (-1 for rows that were skipped). */
+int vk_pages_extend(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page,
+                    const int32_t* list, int n, int count, int32_t* page_out, int32_t* slot_out, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Rows dst[i] become copies of rows src[i] as they were before the call, i < n: full pages are shared, a partly filled
+ * last page is copied in all layers (k, v [layers, n_pages, page, token_bytes], token_bytes a multiple of 16).  What a
+ * dst row held before is released; a page released by a call is given out from the next call on. */
+int vk_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page,
+                  const int32_t* src, const int32_t* dst, int n, void* k, void* v, int layers, int token_bytes,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* The rows list[0 .. n) (NULL: all rows, n = rows) release their pages and are empty.  A row may be named twice. */
+int vk_pages_free(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages,
+                  const int32_t* list, int n, void* stream);
+
+/* Moves pages in use until they are the lowest ones: with L = the pages in use (written to live [1] i32), those
+ * numbered L and above go into the free pages below L, both in ascending order; table and refs follow. */
+int vk_pages_compact(int32_t* table, int32_t* refs, int rows, int max_pages, int n_pages, int page, void* k, void* v,
+                     int layers, int token_bytes, int32_t* live, void* workspace, size_t workspace_bytes, void* stream);
+
+/* logits [B, V] (VK_F32, VK_BF16 or VK_F16, row stride ld) -> out (same type, row stride ld_out; may be logits itself):
+ * with c = the times v stands in history[b, 0 .. history_lens[b]) (i64, row stride ld_history, T columns; ids outside
+ * 0..V-1 are passed over), l = c ? (logit > 0 ? logit / repetition[b] : logit * repetition[b]) : logit and
+ * out = l - frequency[b] * c - presence[b] * (c > 0) + bias[b * ld_bias + v], or -inf where the grammar mask has a 0:
+ * bit v % 32 of word mask[m * ld_mask + v / 32], m = mask_index[b] (i32; -1: no mask), or without mask_index m = b, or 0
+ * where masks is 1.  history with its lengths, repetition, presence, frequency ([B] f32), bias (f32; ld_bias 0: one
+ * for all rows) and mask may each be NULL. */
+int vk_penalize_logits(const void* logits, void* out, int dtype, int64_t ld, int64_t ld_out, int B, int V,
+                       const int64_t* history, const int32_t* history_lens, int T, int64_t ld_history,
+                       const float* repetition, const float* presence, const float* frequency, const float* bias,
+                       int64_t ld_bias, const uint32_t* mask, int64_t ld_mask, int masks, const int32_t* mask_index,
+                       void* stream);
 
 /* ---- host-side stitching of chunk calls (scripts/basecall_viktor.py:31-108; no device work) -----------------
  * Edit-distance alignment with edlib's semantics (the reference's aligner): mode 0 NW (global), 1 SHW (query

@@ -13,7 +13,8 @@ _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "li
 VK_OK, VK_ERR_ARG, VK_ERR_CUDA, VK_ERR_UNSUPPORTED = 0, -1, -2, -3
 _STATUS = {VK_ERR_ARG: "bad argument", VK_ERR_CUDA: "CUDA error", VK_ERR_UNSUPPORTED: "unsupported geometry"}
 DEVERR = {1: "wait for a TMA stage timed out", 2: "wait for a free stage timed out",
-          4: "wait for the tensor-core accumulator timed out", 8: "index out of range (access skipped)"}
+          4: "wait for the tensor-core accumulator timed out", 8: "index out of range (access skipped)",
+          16: "no free cache page (row not changed)"}
 
 p, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 
@@ -42,6 +43,15 @@ _SIGS = {
     "vk_decode_attention_i8_workspace_bytes": (sz, [i32, i32, i32]),
     "vk_decode_attention_i8": (i32, [p, p, p, p, p, p, p, p, p, p, i32, i32, i32, i32, i64, i64, i32, i32, p, sz,
                                      p]),
+    "vk_shared_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
+    "vk_shared_attention": (i32, [p, i64, i32, p, p, p, p, i32, i32, i64, i64, p, p, i32, i32, i64, p, i32, i64, p, p, p, i32,
+                                  i32, i32, i32, f32, p, sz, p]),
+    "vk_pages_workspace_bytes": (sz, [i32, i32, i32, i32]),
+    "vk_pages_extend": (i32, [p, p, p, i32, i32, i32, i32, p, i32, i32, p, p, p, sz, p]),
+    "vk_pages_fork": (i32, [p, p, p, i32, i32, i32, i32, p, p, i32, p, p, i32, i32, p, sz, p]),
+    "vk_pages_free": (i32, [p, p, p, i32, i32, i32, p, i32, p]),
+    "vk_pages_compact": (i32, [p, p, i32, i32, i32, i32, p, p, i32, i32, p, p, sz, p]),
+    "vk_penalize_logits": (i32, [p, p, i32, i64, i64, i32, i32, p, p, i32, i64, p, p, p, p, i64, p, i64, i32, p, p]),
     "vk_align": (i32, [p, i32, p, i32, i32, i32, p, p, i32]),
     "vk_overlap_cut": (i32, [p, i32, p, i32, i32, C.c_double, p]),
     "vk_stitch": (i32, [p, p, p, i32, i32, p, i64, p]),
@@ -64,8 +74,10 @@ _SIGS = {
 
 _lib = None
 _HOST_ONLY = {"vk_version", "vk_read_device_errors", "vk_set_pdl", "vk_decode_attention_workspace_bytes",
-              "vk_decode_attention_i8_workspace_bytes", "vk_align", "vk_overlap_cut", "vk_stitch"}
-launches = 0  # kernels launched through call() (each launching entry point launches exactly one kernel)
+              "vk_decode_attention_i8_workspace_bytes", "vk_align", "vk_overlap_cut", "vk_stitch",
+              "vk_shared_attention_workspace_bytes", "vk_pages_workspace_bytes"}
+_KERNELS = {"vk_pages_fork": 2, "vk_pages_compact": 2}  # kernels of one call where it is not one
+launches = 0  # kernels launched through call()
 
 
 def lib_path() -> str:
@@ -98,7 +110,7 @@ def call(name: str, *args):
     if rc != VK_OK:
         raise RuntimeError(f"{name} failed: {_STATUS.get(rc, rc)}")
     if name not in _HOST_ONLY:
-        launches += 1
+        launches += _KERNELS.get(name, 1)
     return rc
 
 

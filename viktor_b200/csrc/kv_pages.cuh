@@ -1,0 +1,343 @@
+// Pages of a KV cache: rows of a table name pages of a pool, refs counts the rows that name a page.
+//
+// A page is free while its count is zero.  All but the last page of a row are full, and only full pages are shared:
+// a fork copies the partly filled last page, so a row may always write behind its last token.  Pages are given out the
+// lowest first, in the order of the request, so that equal requests give equal tables.
+//
+// The bookkeeping (whole numbers, a few KB to a few hundred KB) runs in one CTA whose phases are separated by block
+// barriers; the copies run in a second kernel over all SMs.
+#pragma once
+
+#include "vk_common.cuh"
+
+namespace vk {
+namespace pages {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kCopyThreads = 256;
+
+struct Pool {
+  int32_t* table;  // [rows, max_pages], -1 behind a row's last page
+  int32_t* lens;   // [rows] tokens
+  int32_t* refs;   // [n_pages]
+  int rows, max_pages, n_pages, page_shift;
+};
+
+struct Move {
+  int32_t src, dst, tokens;  // tokens 0: nothing to copy
+};
+
+// Exclusive prefix sum of one value per thread over the block; *total gets the sum.  All threads of the block call it.
+VK_DEV int block_scan(int v, int* total) {
+  __shared__ int warp_sums[kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, off);
+    if (lane >= off) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    const int s = warp_sums[w];
+    before += w < warp ? s : 0;
+    all += s;
+  }
+  __syncthreads();  // warp_sums may be written again
+  *total = all;
+  return before + x - v;
+}
+
+// The lowest `want` free pages into list; returns how many there are (at most want).
+VK_DEV int free_pages(const Pool& p, int want, int32_t* list) {
+  int found = 0;
+  for (int base = 0; base < p.n_pages && found < want; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    const int is_free = i < p.n_pages && p.refs[i] <= 0;
+    int n;
+    const int at = found + block_scan(is_free, &n);
+    if (is_free && at < want) list[at] = i;
+    found += n;
+  }
+  __syncthreads();
+  return found < want ? found : want;
+}
+
+// Which of the items naming row (one item per thread) has it: the first in the list.  claim: [rows] scratch.
+VK_DEV void claim_rows(const int32_t* list, int n, int rows, int32_t* claim) {
+  for (int i = threadIdx.x; i < n; i += kPlanThreads)
+    if (list[i] >= 0 && list[i] < rows) claim[list[i]] = 0x7fffffff;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kPlanThreads)
+    if (list[i] >= 0 && list[i] < rows) atomicMin(&claim[list[i]], i);
+  __syncthreads();
+}
+
+VK_DEV int row_len(const Pool& p, int row) {
+  const int len = p.lens[row], most = p.max_pages << p.page_shift;
+  if (len >= 0 && len <= most) return len;
+  raise_error(ERR_BOUNDS);
+  return len < 0 ? 0 : most;
+}
+VK_DEV int pages_of(const Pool& p, int len) { return (len + (1 << p.page_shift) - 1) >> p.page_shift; }
+
+struct ExtendArgs {
+  Pool p;
+  const int32_t* list;  // [n] rows, or NULL: all rows
+  int n, count;
+  int32_t* page;        // [n, count] out
+  int32_t* slot;
+  int32_t* claim;       // [rows] scratch
+  int32_t* first;       // [n] scratch: place of the item's first new page in the free list, -1: not served
+  int32_t* free_list;   // [n_pages] scratch
+};
+
+// Room for `count` more tokens in each listed row.
+__global__ void __launch_bounds__(kPlanThreads) extend_kernel(ExtendArgs a) {
+  const Pool& p = a.p;
+  pdl_wait();
+  if (a.list) claim_rows(a.list, a.n, p.rows, a.claim);
+  int want = 0;
+  for (int base = 0; base < a.n; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0;
+    bool ok = i < a.n;
+    if (ok) {
+      const int row = a.list ? a.list[i] : i;
+      ok = row >= 0 && row < p.rows && (!a.list || a.claim[row] == i);
+      if (ok) {
+        const int len = row_len(p, row);
+        ok = len + a.count <= p.max_pages << p.page_shift;
+        if (ok) need = pages_of(p, len + a.count) - pages_of(p, len);
+      }
+      if (!ok) raise_error(ERR_BOUNDS);
+    }
+    int n;
+    const int at = want + block_scan(need, &n);
+    if (i < a.n) a.first[i] = ok ? at : -1;
+    want += n;
+  }
+  const int got = free_pages(p, want < p.n_pages ? want : p.n_pages, a.free_list);
+  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
+    const int row = a.list ? a.list[i] : i, at = a.first[i];
+    int len = 0, old = 0;
+    bool ok = at >= 0;
+    if (ok) {
+      len = row_len(p, row);
+      old = pages_of(p, len);
+      const int need = pages_of(p, len + a.count) - old;
+      ok = need == 0 || at + need <= got;
+      if (!ok) raise_error(ERR_PAGES);
+    }
+    if (!ok) {
+      for (int j = 0; j < a.count; ++j) a.page[static_cast<int64_t>(i) * a.count + j] = a.slot[static_cast<int64_t>(i) * a.count + j] = -1;
+      continue;
+    }
+    int32_t* t = p.table + static_cast<int64_t>(row) * p.max_pages;
+    for (int j = 0; j < a.count; ++j) {
+      const int pos = len + j, c = pos >> p.page_shift;
+      int pg;
+      if (c < old) {
+        pg = t[c];
+      } else {
+        pg = a.free_list[at + c - old];
+        t[c] = pg;
+        p.refs[pg] = 1;
+      }
+      a.page[static_cast<int64_t>(i) * a.count + j] = pg;
+      a.slot[static_cast<int64_t>(i) * a.count + j] = pos & ((1 << p.page_shift) - 1);
+    }
+    p.lens[row] = len + a.count;
+  }
+}
+
+struct ForkArgs {
+  Pool p;
+  const int32_t* src;
+  const int32_t* dst;
+  int n;
+  int32_t* claim;      // [rows] scratch
+  int32_t* state;      // [n] scratch: place in the free list, -1: not served or nothing to do
+  int32_t* len;        // [n] scratch: the new length
+  int32_t* stage;      // [n, max_pages] scratch: the new table rows
+  int32_t* free_list;  // [n] scratch
+  Move* moves;         // [n] out
+};
+
+// Rows dst[i] become copies of the rows src[i] as they were before the call.
+__global__ void __launch_bounds__(kPlanThreads) fork_kernel(ForkArgs a) {
+  const Pool& p = a.p;
+  const int mask = (1 << p.page_shift) - 1;
+  pdl_wait();
+  claim_rows(a.dst, a.n, p.rows, a.claim);
+  int want = 0;
+  for (int base = 0; base < a.n; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0;
+    bool ok = i < a.n;
+    if (ok) {
+      const int s = a.src[i], t = a.dst[i];
+      ok = s >= 0 && s < p.rows && t >= 0 && t < p.rows && a.claim[t] == i;
+      if (!ok) raise_error(ERR_BOUNDS);
+      if (ok && s == t) ok = false;
+      if (ok) {
+        a.len[i] = row_len(p, s);
+        need = (a.len[i] & mask) != 0;
+      }
+    }
+    int n;
+    const int at = want + block_scan(need, &n);
+    if (i < a.n) a.state[i] = ok ? at : -1;
+    want += n;
+  }
+  const int got = free_pages(p, want, a.free_list);
+  // the new table rows, and what is copied
+  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
+    Move m{0, 0, 0};
+    const int at = a.state[i];
+    if (at >= 0) {
+      const int part = a.len[i] & mask, full = a.len[i] >> p.page_shift;
+      if (part && at >= got) {
+        raise_error(ERR_PAGES);
+        a.state[i] = -1;
+      } else if (part) {
+        const int from = p.table[static_cast<int64_t>(a.src[i]) * p.max_pages + full];
+        if (from >= 0 && from < p.n_pages)
+          m = Move{from, a.free_list[at], part};
+        else
+          raise_error(ERR_BOUNDS);
+      }
+    }
+    a.moves[i] = m;
+  }
+  __syncthreads();
+  const int64_t cells = static_cast<int64_t>(a.n) * p.max_pages;
+  for (int64_t x = threadIdx.x; x < cells; x += kPlanThreads) {
+    const int i = static_cast<int>(x / p.max_pages), c = static_cast<int>(x % p.max_pages), at = a.state[i];
+    if (at < 0) continue;
+    const int full = a.len[i] >> p.page_shift;
+    int v = -1;
+    if (c < full)
+      v = p.table[static_cast<int64_t>(a.src[i]) * p.max_pages + c];
+    else if (c == full && (a.len[i] & mask))
+      v = a.free_list[at];
+    a.stage[x] = v;
+  }
+  __syncthreads();
+  for (int64_t x = threadIdx.x; x < cells; x += kPlanThreads) {
+    const int i = static_cast<int>(x / p.max_pages), c = static_cast<int>(x % p.max_pages);
+    if (a.state[i] < 0) continue;
+    int32_t* cell = p.table + static_cast<int64_t>(a.dst[i]) * p.max_pages + c;
+    const int old = *cell, now = a.stage[x];
+    if (old >= 0 && old < p.n_pages) atomicSub(&p.refs[old], 1);
+    if (now >= 0 && now < p.n_pages) atomicAdd(&p.refs[now], 1);
+    *cell = now;
+    if (c == 0) p.lens[a.dst[i]] = a.len[i];
+  }
+}
+
+// The listed rows (NULL: all) give their pages up.  One warp per row; a row named twice is empty the second time.
+__global__ void __launch_bounds__(256) free_kernel(Pool p, const int32_t* list, int n) {
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  pdl_wait();
+  if (i >= n) return;
+  const int row = list ? list[i] : i;
+  if (row < 0 || row >= p.rows) {
+    if (lane == 0) raise_error(ERR_BOUNDS);
+    return;
+  }
+  if (lane == 0) p.lens[row] = 0;
+  for (int c = lane; c < p.max_pages; c += 32) {
+    const int old = atomicExch(&p.table[static_cast<int64_t>(row) * p.max_pages + c], -1);
+    if (old >= 0 && old < p.n_pages) atomicSub(&p.refs[old], 1);
+  }
+}
+
+struct CompactArgs {
+  Pool p;
+  int32_t* holes;   // [n_pages] scratch
+  int32_t* goes;    // [n_pages] scratch: where a moved page goes
+  Move* moves;      // [n_pages / 2] out
+  int32_t* counts;  // [1] out: moves
+  int32_t* live;    // [1] out: pages in use
+};
+
+// The live pages from number `live` on go into the free pages below it, both in ascending order.
+__global__ void __launch_bounds__(kPlanThreads) compact_kernel(CompactArgs a) {
+  const Pool& p = a.p;
+  pdl_wait();
+  int live = 0;
+  for (int base = 0; base < p.n_pages; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int n;
+    block_scan(i < p.n_pages && p.refs[i] > 0, &n);
+    live += n;
+  }
+  int holes = 0;
+  for (int base = 0; base < live; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    const int is = i < live && p.refs[i] <= 0;
+    int n;
+    const int at = holes + block_scan(is, &n);
+    if (is) a.holes[at] = i;
+    holes += n;
+  }
+  __syncthreads();
+  int moved = 0;
+  for (int base = live; base < p.n_pages; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    const int is = i < p.n_pages && p.refs[i] > 0;
+    int n;
+    const int at = moved + block_scan(is, &n);
+    if (is) {
+      const int to = a.holes[at];
+      a.moves[at] = Move{i, to, 1 << p.page_shift};
+      a.goes[i] = to;
+      p.refs[to] = p.refs[i];
+      p.refs[i] = 0;
+    }
+    moved += n;
+  }
+  __syncthreads();
+  const int64_t cells = static_cast<int64_t>(p.rows) * p.max_pages;
+  for (int64_t x = threadIdx.x; x < cells; x += kPlanThreads) {
+    const int old = p.table[x];
+    if (old >= live && old < p.n_pages) p.table[x] = a.goes[old];
+  }
+  if (threadIdx.x == 0) {
+    a.counts[0] = moved;
+    a.live[0] = live;
+  }
+}
+
+struct CopyArgs {
+  uint8_t* k;          // [layers, n_pages, page_bytes]
+  uint8_t* v;
+  const Move* moves;
+  const int32_t* count;  // moves to make, or NULL: n
+  int n, layers;
+  int64_t page_bytes, layer_bytes;
+  int token_bytes;     // a multiple of 16
+};
+
+// Copies each move's tokens in every layer of K and V.
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(CopyArgs a) {
+  pdl_wait();
+  const int n = a.count ? *a.count : a.n;
+  const int64_t units = static_cast<int64_t>(n) * a.layers * 2;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const Move m = a.moves[u / (a.layers * 2)];
+    const int layer = static_cast<int>(u / 2 % a.layers);
+    uint8_t* base = (u & 1 ? a.v : a.k) + layer * a.layer_bytes;
+    const uint4* from = reinterpret_cast<const uint4*>(base + m.src * a.page_bytes);
+    uint4* to = reinterpret_cast<uint4*>(base + m.dst * a.page_bytes);
+    const int64_t words = static_cast<int64_t>(m.tokens) * a.token_bytes / 16;
+    for (int64_t i = threadIdx.x; i < words; i += kCopyThreads) to[i] = from[i];
+  }
+}
+
+}  // namespace pages
+}  // namespace vk

@@ -7,7 +7,10 @@
 #include "decode_attention.cuh"
 #include "elementwise.cuh"
 #include "gemm_tc.cuh"
+#include "kv_pages.cuh"
+#include "logit_penalties.cuh"
 #include "prefill_attention.cuh"
+#include "shared_attention.cuh"
 #include "stitch_host.h"
 #include "vk_host.cuh"
 
@@ -89,6 +92,12 @@ static int device_sm_count() {
 }
 
 static inline unsigned blocks_for(int64_t n, int per) { return static_cast<unsigned>((n + per - 1) / per); }
+
+static inline int log2_of(int power) {
+  int k = 0;
+  while ((1 << k) < power) ++k;
+  return k;
+}
 
 constexpr int64_t kSmallM = 4096;  // decode-sized GEMMs: narrow tiles + split-K clusters; prefill: wide tiles
 
@@ -871,6 +880,229 @@ int vk_scatter_embed(void* x, const int64_t* rows, int64_t n, int64_t x_rows, co
     return VK_ERR_ARG;
   return launch(ew::scatter_embed_kernel, dim3(static_cast<unsigned>(n)), dim3(64), 0, stream, 1,
                 static_cast<__nv_bfloat16*>(x), rows, n, x_rows, static_cast<const __nv_bfloat16*>(emb), token, d);
+}
+
+// ---- several candidates of a chunk ------------------------------------------------------------------------------
+size_t vk_shared_attention_workspace_bytes(int B, int H, int HK, int D, int P, int S, int max_tail) {
+  if (B <= 0 || H <= 0 || HK <= 0 || D <= 0 || P <= 0 || S <= 0 || max_tail < 0) return 0;
+  return 16;
+}
+
+int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* k_prefix, const void* v_prefix,
+                        const int32_t* prefix_lens, const int32_t* group_offsets, int P, int S, int64_t stride_kb,
+                        int64_t stride_ks, const void* k_pages, const void* v_pages, int n_pages, int page,
+                        int64_t stride_pp, const int32_t* page_table, int max_pages, int64_t stride_table,
+                        const int32_t* tail_lens, void* out, float* lse, int B, int H, int HK, int D, float scale,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (B == 0) return VK_OK;
+  if (B < 0 || P <= 0 || S <= 0 || H <= 0 || HK <= 0 || H % HK || n_pages <= 0 || max_pages < 0 || page < 8 ||
+      page > 256 || (page & (page - 1)) || !(scale > 0.f) || !(scale < INFINITY))
+    return VK_ERR_ARG;
+  if ((D != 64 && D != 128) || (dtype != VK_BF16 && dtype != VK_F16)) return VK_ERR_UNSUPPORTED;
+  if (!q || !k_prefix || !v_prefix || !prefix_lens || !group_offsets || !k_pages || !v_pages || !tail_lens || !out ||
+      !workspace || (max_pages && !page_table))
+    return VK_ERR_ARG;
+  const int64_t token = static_cast<int64_t>(HK) * D, cap = int64_t(1) << 31;
+  if (static_cast<int64_t>(B) * H >= cap || static_cast<int64_t>(max_pages) * page + S >= cap ||
+      stride_q < static_cast<int64_t>(H) * D || stride_q % 8 || stride_ks < token || stride_ks % 8 ||
+      stride_kb < stride_ks * S || stride_kb % 8 || stride_pp < token * page || stride_pp % 8 ||
+      stride_table < max_pages)
+    return VK_ERR_ARG;
+  if (!aligned16(q) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(k_pages) || !aligned16(v_pages) ||
+      !aligned16(out) || !aligned16(workspace) ||
+      workspace_bytes < vk_shared_attention_workspace_bytes(B, H, HK, D, P, S, max_pages * page))
+    return VK_ERR_ARG;
+  sattn::Args a;
+  memset(&a, 0, sizeof(a));
+  a.q = q;
+  a.k_prefix = k_prefix;
+  a.v_prefix = v_prefix;
+  a.prefix_lens = prefix_lens;
+  a.offsets = group_offsets;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.table = page_table;
+  a.tail_lens = tail_lens;
+  a.out = out;
+  a.lse = lse;
+  a.stride_q = stride_q;
+  a.stride_kb = stride_kb;
+  a.stride_ks = stride_ks;
+  a.stride_pp = stride_pp;
+  a.stride_table = stride_table;
+  a.B = B;
+  a.H = H;
+  a.HK = HK;
+  a.P = P;
+  a.S = S;
+  a.n_pages = n_pages;
+  a.page_shift = log2_of(page);
+  a.max_pages = max_pages;
+  a.scale = scale;
+  void (*kern)(sattn::Args) = nullptr;
+  if (dtype == VK_BF16)
+    kern = D == 64 ? sattn::rows_kernel<__nv_bfloat16, 64> : sattn::rows_kernel<__nv_bfloat16, 128>;
+  else
+    kern = D == 64 ? sattn::rows_kernel<__half, 64> : sattn::rows_kernel<__half, 128>;
+  return launch(kern, dim3(blocks_for(static_cast<int64_t>(B) * H, 4)), dim3(128), 0, stream, 1, a);
+}
+
+// Scratch of the page calls, one region after another: ints, then the moves.
+static size_t pages_ints(int rows, int max_pages, int n_pages, int n) {
+  return static_cast<size_t>(rows) + 2 * static_cast<size_t>(n_pages) + 3 * static_cast<size_t>(n) +
+         static_cast<size_t>(n) * max_pages + 4;
+}
+size_t vk_pages_workspace_bytes(int rows, int max_pages, int n_pages, int n) {
+  if (rows <= 0 || max_pages <= 0 || n_pages <= 0 || n < 0) return 0;
+  return 4 * pages_ints(rows, max_pages, n_pages, n) + sizeof(pages::Move) * (static_cast<size_t>(n) + n_pages / 2 + 1);
+}
+
+static bool pool_ok(const int32_t* table, const int32_t* refs, int rows, int max_pages, int n_pages, int page) {
+  return table && refs && rows > 0 && max_pages > 0 && n_pages > 0 && page >= 8 && page <= 256 && !(page & (page - 1)) &&
+         static_cast<int64_t>(rows) * max_pages < (int64_t(1) << 31) &&
+         static_cast<int64_t>(max_pages) * page < (int64_t(1) << 31);
+}
+static pages::Pool pool_of(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page) {
+  return pages::Pool{table, lens, refs, rows, max_pages, n_pages, log2_of(page)};
+}
+
+int vk_pages_extend(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page,
+                    const int32_t* list, int n, int count, int32_t* page_out, int32_t* slot_out, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  if (n == 0) return VK_OK;
+  if (!pool_ok(table, refs, rows, max_pages, n_pages, page) || !lens || n < 0 || (!list && n != rows) || count <= 0 ||
+      count > max_pages * page || !page_out || !slot_out || !workspace || !aligned16(workspace) ||
+      workspace_bytes < vk_pages_workspace_bytes(rows, max_pages, n_pages, n))
+    return VK_ERR_ARG;
+  pages::ExtendArgs a;
+  a.p = pool_of(table, lens, refs, rows, max_pages, n_pages, page);
+  a.list = list;
+  a.n = n;
+  a.count = count;
+  a.page = page_out;
+  a.slot = slot_out;
+  a.claim = static_cast<int32_t*>(workspace);
+  a.first = a.claim + rows;
+  a.free_list = a.first + n;
+  return launch(pages::extend_kernel, dim3(1), dim3(pages::kPlanThreads), 0, stream, 1, a);
+}
+
+static int copy_pages(const pages::CopyArgs& c, int64_t most, void* stream) {
+  const int sms = device_sm_count();
+  if (sms <= 0) return VK_ERR_CUDA;
+  const int64_t units = most * c.layers * 2;
+  return launch(pages::copy_kernel, dim3(static_cast<unsigned>(units < 8 * sms ? units : 8 * sms)),
+                dim3(pages::kCopyThreads), 0, stream, 1, c);
+}
+
+int vk_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page,
+                  const int32_t* src, const int32_t* dst, int n, void* k, void* v, int layers, int token_bytes,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (n == 0) return VK_OK;
+  if (!pool_ok(table, refs, rows, max_pages, n_pages, page) || !lens || n < 0 || !src || !dst || !k || !v ||
+      layers <= 0 || token_bytes <= 0 || token_bytes % 16 || !aligned16(k) || !aligned16(v) || !workspace ||
+      !aligned16(workspace) || workspace_bytes < vk_pages_workspace_bytes(rows, max_pages, n_pages, n) ||
+      static_cast<int64_t>(n) * max_pages >= (int64_t(1) << 31))
+    return VK_ERR_ARG;
+  pages::ForkArgs a;
+  a.p = pool_of(table, lens, refs, rows, max_pages, n_pages, page);
+  a.src = src;
+  a.dst = dst;
+  a.n = n;
+  a.claim = static_cast<int32_t*>(workspace);
+  a.state = a.claim + rows;
+  a.len = a.state + n;
+  a.free_list = a.len + n;
+  a.stage = a.free_list + n;
+  a.moves = reinterpret_cast<pages::Move*>(static_cast<int32_t*>(workspace) + pages_ints(rows, max_pages, n_pages, n));
+  const int rc = launch(pages::fork_kernel, dim3(1), dim3(pages::kPlanThreads), 0, stream, 1, a);
+  if (rc != VK_OK) return rc;
+  pages::CopyArgs c;
+  c.k = static_cast<uint8_t*>(k);
+  c.v = static_cast<uint8_t*>(v);
+  c.moves = a.moves;
+  c.count = nullptr;
+  c.n = n;
+  c.layers = layers;
+  c.token_bytes = token_bytes;
+  c.page_bytes = static_cast<int64_t>(token_bytes) * page;
+  c.layer_bytes = c.page_bytes * n_pages;
+  return copy_pages(c, n, stream);
+}
+
+int vk_pages_free(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages,
+                  const int32_t* list, int n, void* stream) {
+  if (n == 0) return VK_OK;
+  if (!pool_ok(table, refs, rows, max_pages, n_pages, 8) || !lens || n < 0 || (!list && n != rows)) return VK_ERR_ARG;
+  return launch(pages::free_kernel, dim3(blocks_for(n, 8)), dim3(256), 0, stream, 1,
+                pool_of(table, lens, refs, rows, max_pages, n_pages, 8), list, n);
+}
+
+int vk_pages_compact(int32_t* table, int32_t* refs, int rows, int max_pages, int n_pages, int page, void* k, void* v,
+                     int layers, int token_bytes, int32_t* live, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!pool_ok(table, refs, rows, max_pages, n_pages, page) || !k || !v || layers <= 0 || token_bytes <= 0 ||
+      token_bytes % 16 || !aligned16(k) || !aligned16(v) || !live || !workspace || !aligned16(workspace) ||
+      workspace_bytes < vk_pages_workspace_bytes(rows, max_pages, n_pages, 0))
+    return VK_ERR_ARG;
+  pages::CompactArgs a;
+  a.p = pool_of(table, nullptr, refs, rows, max_pages, n_pages, page);
+  a.counts = static_cast<int32_t*>(workspace);
+  a.holes = a.counts + 4;
+  a.goes = a.holes + n_pages;
+  a.moves = reinterpret_cast<pages::Move*>(static_cast<int32_t*>(workspace) + pages_ints(rows, max_pages, n_pages, 0));
+  a.live = live;
+  const int rc = launch(pages::compact_kernel, dim3(1), dim3(pages::kPlanThreads), 0, stream, 1, a);
+  if (rc != VK_OK) return rc;
+  pages::CopyArgs c;
+  c.k = static_cast<uint8_t*>(k);
+  c.v = static_cast<uint8_t*>(v);
+  c.moves = a.moves;
+  c.count = a.counts;
+  c.n = 0;
+  c.layers = layers;
+  c.token_bytes = token_bytes;
+  c.page_bytes = static_cast<int64_t>(token_bytes) * page;
+  c.layer_bytes = c.page_bytes * n_pages;
+  return copy_pages(c, n_pages / 2 + 1, stream);
+}
+
+int vk_penalize_logits(const void* logits, void* out, int dtype, int64_t ld, int64_t ld_out, int B, int V,
+                       const int64_t* history, const int32_t* history_lens, int T, int64_t ld_history,
+                       const float* repetition, const float* presence, const float* frequency, const float* bias,
+                       int64_t ld_bias, const uint32_t* mask, int64_t ld_mask, int masks, const int32_t* mask_index,
+                       void* stream) {
+  if (B == 0) return VK_OK;
+  if (dtype < VK_BF16 || dtype > VK_F32) return VK_ERR_UNSUPPORTED;
+  if (B < 0 || V <= 0 || !logits || !out || ld < V || ld_out < V || (history && (!history_lens || T < 0 || ld_history < T)) ||
+      (bias && ld_bias != 0 && ld_bias < V))
+    return VK_ERR_ARG;
+  if (mask && (masks <= 0 || ld_mask < (V + 31) / 32 || (!mask_index && masks != 1 && masks != B))) return VK_ERR_ARG;
+  const int64_t slices = (V + logit::kSlice - 1) / logit::kSlice;
+  if (slices * B >= (int64_t(1) << 31)) return VK_ERR_ARG;
+  logit::Args a;
+  a.logits = logits;
+  a.out = out;
+  a.ld = ld;
+  a.ld_out = ld_out;
+  a.history = T > 0 ? history : nullptr;
+  a.history_lens = history_lens;
+  a.ld_history = ld_history;
+  a.repetition = repetition;
+  a.presence = presence;
+  a.frequency = frequency;
+  a.bias = bias;
+  a.ld_bias = ld_bias;
+  a.mask = mask;
+  a.ld_mask = ld_mask;
+  a.mask_index = mask_index;
+  a.masks = masks;
+  a.B = B;
+  a.V = V;
+  a.T = T;
+  auto kern = dtype == VK_F32    ? logit::penalize_kernel<float>
+              : dtype == VK_BF16 ? logit::penalize_kernel<__nv_bfloat16>
+                                 : logit::penalize_kernel<__half>;
+  return launch(kern, dim3(static_cast<unsigned>(slices * B)), dim3(logit::kThreads), 0, stream, 1, a);
 }
 
 // ---- host-side stitching (no device work) ------------------------------------------------------------------

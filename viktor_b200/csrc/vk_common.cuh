@@ -21,6 +21,7 @@ enum ErrBits : uint32_t {
   ERR_WAIT_EMPTY = 1u << 1,   // producer gave up waiting for a free stage
   ERR_WAIT_ACCUM = 1u << 2,   // epilogue gave up waiting for the MMA accumulator
   ERR_BOUNDS = 1u << 3,       // an index failed its range check and the access was skipped
+  ERR_PAGES = 1u << 4,        // no free cache page was left; the row was not changed
 };
 
 __device__ uint32_t g_error_word = 0;  // single translation unit: defined once here
@@ -339,5 +340,42 @@ VK_DEV uint32_t pack_bf16x2(float lo, float hi) {
 }
 VK_DEV float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 VK_DEV float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+// ---- element types ---------------------------------------------------------------------------------------------
+template <typename T>
+VK_DEV float to_f32(T x);
+template <>
+VK_DEV float to_f32(__nv_bfloat16 x) {
+  return __bfloat162float(x);
+}
+template <>
+VK_DEV float to_f32(__half x) {
+  return __half2float(x);
+}
+template <>
+VK_DEV float to_f32(float x) {
+  return x;
+}
+template <typename T>
+VK_DEV T from_f32(float x);
+template <>
+VK_DEV __nv_bfloat16 from_f32(float x) {
+  return __float2bfloat16_rn(x);
+}
+template <>
+VK_DEV __half from_f32(float x) {
+  return __float2half_rn(x);
+}
+template <>
+VK_DEV float from_f32(float x) {
+  return x;
+}
+
+// Length v clamped to 0..most; a length outside is reported.
+VK_DEV int checked_len(int v, int most) {
+  if (v >= 0 && v <= most) return v;
+  raise_error(ERR_BOUNDS);
+  return v < 0 ? 0 : most;
+}
 
 }  // namespace vk

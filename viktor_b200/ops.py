@@ -287,3 +287,255 @@ def gather_rows(src, idx, out=None):
 def scatter_embed(x, rows, emb, token):
     call("vk_scatter_embed", _p(x), _p(rows), rows.shape[0], x.shape[0], _p(emb), int(token), x.shape[1],
          _stream(x))
+
+
+# ---------------------------------------------------------------- several candidates of a chunk (no reference counterpart)
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_I32 = torch.int32
+
+
+def _launch(name, device, *args):
+    """call() on the current stream of `device`, which need not be the current device."""
+    if device.type != "cuda":
+        raise ValueError("viktor_b200 ops need CUDA tensors (there is no CPU path)")
+    if device.index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _same_device(*ts):
+    """The one device of the tensors."""
+    device = ts[0].device
+    for t in ts:
+        _need(t is None or t.device == device, "all tensors must be on one device")
+    return device
+
+
+def _ints(name, t, *shape):
+    _need(t.dtype == _I32 and tuple(t.shape) == shape and t.is_contiguous(), f"{name}: a contiguous int32 {list(shape)}")
+
+
+def _cache_strides(t):
+    """(row stride, position stride) in elements of [P, S, HK, D] whose positions are laid out as [HK, D]."""
+    P, S, HK, D = t.shape
+    sb, ss, sh, sd = t.stride()
+    _need(sd == 1 and (HK == 1 or sh == D), "the last two dimensions of a cache must be contiguous")
+    ss = ss if S > 1 else HK * D
+    return sb if P > 1 else ss * S, ss
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k_pages, v_pages, page_table, tail_lens,
+                            scale=None, out=None, return_lse=False, workspace=None):
+    """Attention of one query token per row over a prefix that a group of rows shares and the row's own tail.
+
+    q [B, H, D] bf16 or fp16 (D 64 or 128); k_prefix / v_prefix [P, S, HK, D]: one layer of a static cache, one row per
+    group; prefix_lens [P] int32; group_offsets [P + 1] int32: rows group_offsets[g] .. group_offsets[g + 1] - 1 belong
+    to group g.  k_pages / v_pages [n_pages, page, HK, D]: one layer of a KVPages; page_table [B, max_pages] int32;
+    tail_lens [B] int32.  Query head h reads KV head h // (H // HK).  scale: 1 / sqrt(D) by default.
+
+    Returns out [B, H, D], with return_lse also the log of the sum of exponentials [B, H] (float32).  A row with nothing
+    to attend gets 0 and -inf; rows behind the last group are not written.  What a cache holds behind a length is not
+    used.  workspace: uint8, vk_shared_attention_workspace_bytes; calls that may run at the same time need one each (by
+    default every call allocates its own)."""
+    _need(q.dim() == 3 and k_prefix.dim() == 4 and k_pages.dim() == 4, "q [B, H, D], caches of four dimensions")
+    B, H, D = q.shape
+    P, S, HK, _ = k_prefix.shape
+    n_pages, page = k_pages.shape[:2]
+    device = _same_device(q, k_prefix, v_prefix, prefix_lens, group_offsets, k_pages, v_pages, page_table, tail_lens, out,
+                          workspace)
+    dtype = q.dtype
+    _need(dtype in (torch.bfloat16, torch.float16) and k_prefix.dtype == v_prefix.dtype == k_pages.dtype == v_pages.dtype
+          == dtype, "q and the caches must all be bfloat16 or all float16")
+    _need(D in (64, 128), "head_dim must be 64 or 128")
+    _need(P > 0 and S > 0 and HK > 0 and n_pages > 0 and H > 0 and H % HK == 0, "empty cache, or heads that do not divide")
+    _need(page in (8, 16, 32, 64, 128, 256), "pages hold a power of two from 8 to 256 tokens")
+    _need(k_prefix.shape == v_prefix.shape and k_prefix.shape[3] == D, "k_prefix and v_prefix: [P, S, HK, D]")
+    _need(k_pages.shape == v_pages.shape and k_pages.shape[2:] == (HK, D), "k_pages and v_pages: [n_pages, page, HK, D]")
+    _need(page_table.dim() == 2 and page_table.dtype == _I32 and page_table.shape[0] == B, "page_table: int32 [B, max_pages]")
+    max_pages = page_table.shape[1]
+    _need(max_pages < 2 or page_table.stride(1) == 1, "the rows of page_table must be contiguous")
+    stride_table = page_table.stride(0) if B > 1 else max_pages
+    _need(stride_table >= max_pages, "rows of page_table that overlap")
+    _ints("prefix_lens", prefix_lens, P)
+    _ints("group_offsets", group_offsets, P + 1)
+    _ints("tail_lens", tail_lens, B)
+    stride_q = q.stride(0) if B > 1 else H * D
+    _need(stride_q >= H * D and stride_q % 8 == 0, "the rows of q must be 16-byte aligned and must not overlap")
+    _need(q.stride(2) == 1 and (H == 1 or q.stride(1) == D), "the heads of a row of q must be contiguous")
+    kb, ks = _cache_strides(k_prefix)
+    _need((kb, ks) == _cache_strides(v_prefix), "k_prefix and v_prefix must have the same strides")
+    _need(ks >= HK * D and kb >= ks * S and ks % 8 == 0 and kb % 8 == 0, "positions of a cache that overlap or are not 16-byte "
+          "aligned")
+    pp, ps = _cache_strides(k_pages)
+    _need((pp, ps) == _cache_strides(v_pages) and ps == HK * D, "pages must be contiguous, with the same strides in k and v")
+    _need(pp >= page * ps and pp % 8 == 0, "pages that overlap or are not 16-byte aligned")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _need(0.0 < scale < float("inf"), "scale must be positive and finite")
+    if out is None:
+        out = torch.empty(B, H, D, dtype=dtype, device=device)
+    else:
+        _need(out.dtype == dtype and out.shape == q.shape and out.is_contiguous(), "out: contiguous, as q")
+        _need(B == 0 or out.data_ptr() + out.nbytes <= q.data_ptr() or out.data_ptr() >= q.data_ptr() + 2 * (
+            (B - 1) * stride_q + H * D), "out must not overlap q")
+    lse = torch.empty(B, H, dtype=torch.float32, device=device) if return_lse else None
+    if B:
+        nbytes = load().vk_shared_attention_workspace_bytes(B, H, HK, D, P, S, max_pages * page)
+        if workspace is None:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _need(workspace.is_contiguous() and workspace.nbytes >= nbytes, f"workspace: {nbytes} contiguous bytes")
+        _launch("vk_shared_attention", device, _p(q), stride_q, _DTYPES[dtype], _p(k_prefix), _p(v_prefix), _p(prefix_lens),
+                _p(group_offsets), P, S, kb, ks, _p(k_pages), _p(v_pages), n_pages, page, pp, _p(page_table), max_pages,
+                stride_table, _p(tail_lens), _p(out), _p(lse), B, H, HK, D, scale, _p(workspace), workspace.nbytes)
+    return (out, lse) if return_lse else out
+
+
+class KVPages:
+    """Tails of the rows of a decode batch in pages: k / v [layers, n_pages, page, HK, D], table [rows, max_pages] int32 (the
+    pages of each row, -1 behind its last), lens [rows] int32 (tokens of each row), refs [n_pages] int32 (rows that
+    name a page; 0: free).  All but a row's last page are full, and only full pages are shared.  The operations below
+    run on the device without a host wait (they may be captured) and follow one another on one stream."""
+
+    def __init__(self, k, v, table, lens, refs):
+        _need(k.dim() == 5 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
+              "k and v: contiguous [layers, n_pages, page, HK, D] of one type")
+        self.layers, self.n_pages, self.page, hk, d = k.shape
+        self.token_bytes = hk * d * k.element_size()
+        _need(k.numel() > 0 and self.token_bytes % 16 == 0, "a token's K must be a multiple of 16 bytes")
+        _need(self.page in (8, 16, 32, 64, 128, 256), "pages hold a power of two from 8 to 256 tokens")
+        _need(table.dim() == 2 and table.numel() > 0, "table: int32 [rows, max_pages]")
+        self.rows, self.max_pages = table.shape
+        _ints("table", table, self.rows, self.max_pages)
+        _ints("lens", lens, self.rows)
+        _ints("refs", refs, self.n_pages)
+        self.device = _same_device(k, v, table, lens, refs)
+        self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
+
+    @classmethod
+    def empty(cls, layers, n_pages, page, rows, max_pages, n_kv_heads=2, head_dim=64, dtype=_BF16, device="cuda"):
+        """A pool whose pages are all free."""
+        shape = (layers, n_pages, page, n_kv_heads, head_dim)
+        i32 = dict(dtype=_I32, device=device)
+        return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                   torch.full((rows, max_pages), -1, **i32), torch.zeros(rows, **i32), torch.zeros(n_pages, **i32))
+
+    def _workspace(self, n):
+        nbytes = load().vk_pages_workspace_bytes(self.rows, self.max_pages, self.n_pages, n)
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+
+    def _rows(self, name, rows):
+        """(pointer, count) of a list of rows; None stands for all of them."""
+        if rows is None:
+            return None, self.rows
+        _need(rows.dim() == 1 and rows.device == self.device, f"{name}: int32 [n] on the pages' device")
+        _ints(name, rows, rows.shape[0])
+        return rows.data_ptr(), rows.shape[0]
+
+
+def pages_extend(pages: KVPages, count=1, rows=None):
+    """Makes room for `count` more tokens in each of `rows` (int32 [n]; None: all): lens grows, and the tokens' places come
+    back as (page, slot), int32 [n, count] each, to be used as the cache row and position of qkv_rope_cache.  Free pages
+    are taken the lowest first, in the order of the rows.  A row that is out of range, named before, full or for which
+    no page is left is not changed (place -1) and reported by check_device_errors()."""
+    ptr, n = pages._rows("rows", rows)
+    _need(0 < count <= pages.max_pages * pages.page, "count must be 1 to the tokens of a row")
+    page, slot = torch.empty(2, n, count, dtype=_I32, device=pages.device).unbind(0)
+    if n:
+        ws = pages._workspace(n)
+        _launch("vk_pages_extend", pages.device, _p(pages.table), _p(pages.lens), _p(pages.refs), pages.rows, pages.max_pages,
+                pages.n_pages, pages.page, ptr, n, count, _p(page), _p(slot), _p(ws), ws.nbytes)
+    return page, slot
+
+
+def pages_fork(pages: KVPages, src, dst):
+    """Rows dst[i] (int32 [n]) become copies of rows src[i] as they were before the call.  Full pages are shared; a partly
+    filled last page is copied in every layer.  What the dst rows held is released, and given out again from the next
+    call on.  src[i] == dst[i] leaves the row as it is."""
+    src_ptr, n = pages._rows("src", src)
+    dst_ptr, m = pages._rows("dst", dst)
+    _need(src is not None and dst is not None and n == m, "src and dst must have one length")
+    if n:
+        ws = pages._workspace(n)
+        _launch("vk_pages_fork", pages.device, _p(pages.table), _p(pages.lens), _p(pages.refs), pages.rows, pages.max_pages,
+                pages.n_pages, pages.page, src_ptr, dst_ptr, n, _p(pages.k), _p(pages.v), pages.layers, pages.token_bytes,
+                _p(ws), ws.nbytes)
+
+
+def pages_free(pages: KVPages, rows=None):
+    """`rows` (int32 [n]; None: all) give their pages up and are empty."""
+    ptr, n = pages._rows("rows", rows)
+    if n:
+        _launch("vk_pages_free", pages.device, _p(pages.table), _p(pages.lens), _p(pages.refs), pages.rows, pages.max_pages,
+                pages.n_pages, ptr, n)
+
+
+def pages_compact(pages: KVPages):
+    """Moves the pages in use to the lowest numbers: those at or above their count go into the free ones below it, both in
+    ascending order.  Returns the count, int32 [1] on the device."""
+    live = torch.empty(1, dtype=_I32, device=pages.device)
+    ws = pages._workspace(0)
+    _launch("vk_pages_compact", pages.device, _p(pages.table), _p(pages.refs), pages.rows, pages.max_pages, pages.n_pages,
+            pages.page, _p(pages.k), _p(pages.v), pages.layers, pages.token_bytes, _p(live), _p(ws), ws.nbytes)
+    return live
+
+
+def penalize_logits(logits, history=None, history_lens=None, repetition=None, presence=None, frequency=None, bias=None,
+                    mask=None, mask_index=None, out=None):
+    """Penalties for the tokens of each row's history, a bias and a grammar mask, in one pass over the logits [B, V] (float32,
+    bfloat16 or float16; computed in float32, rounded once).
+
+    history [B, T] int64 with history_lens [B] int32: with c = how often v is among the row's first history_lens[b]
+    tokens (ids outside 0..V-1 count for nothing), l = logit / repetition[b] (logit * repetition[b] where it is not
+    positive) if c, then l - frequency[b] * c - presence[b] * (c > 0) + bias ([V] or [B, V]); repetition, presence, frequency
+    and bias float32.  mask [M, ceil(V / 32)] int32: bit v % 32 of word v // 32 is 0 where v is forbidden, which gives -inf
+    whatever the logit holds; mask_index [B] int32 names each row's mask (-1: none), without it M is B or 1.
+    out: as logits (may be logits); returned."""
+    _need(logits.dim() == 2 and logits.dtype in _DTYPES, "logits: float32, bfloat16 or float16 [B, V]")
+    B, V = logits.shape
+    device = _same_device(logits, history, history_lens, repetition, presence, frequency, bias, mask, mask_index, out)
+    _need(V > 0 and (V == 1 or logits.stride(1) == 1), "the rows of logits must be contiguous")
+    if out is None:
+        out = torch.empty(B, V, dtype=logits.dtype, device=device)
+    _need(out.shape == logits.shape and out.dtype == logits.dtype and (V == 1 or out.stride(1) == 1), "out: as logits")
+    ld, ld_out = (t.stride(0) if B > 1 else V for t in (logits, out))
+    _need(ld_out >= V and ld >= V, "rows that overlap")
+    T = ld_history = masks = ld_mask = ld_bias = 0
+    if history is not None:
+        _need(history.dim() == 2 and history.shape[0] == B and history.dtype == torch.int64 and history_lens is not None,
+              "history: int64 [B, T], with history_lens")
+        T = history.shape[1]
+        _need(T < 2 or history.stride(1) == 1, "the rows of history must be contiguous")
+        ld_history = history.stride(0) if B > 1 else T
+        _need(ld_history >= T, "rows that overlap")
+        _ints("history_lens", history_lens, B)
+    else:
+        _need(repetition is None and presence is None and frequency is None, "penalties need a history")
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        _need(t is None or (t.dtype == torch.float32 and t.shape == (B,) and t.is_contiguous()), f"{name}: float32 [B]")
+    if bias is not None:
+        _need(bias.dtype == torch.float32 and bias.shape in ((V,), (B, V)) and (V == 1 or bias.stride(-1) == 1),
+              "bias: float32 [V] or [B, V]")
+        ld_bias = bias.stride(0) if bias.dim() == 2 and B > 1 else 0
+        _need(ld_bias == 0 or ld_bias >= V, "rows that overlap")
+    if mask is not None:
+        _need(mask.dim() == 2 and mask.dtype == _I32 and mask.shape[0] > 0 and mask.shape[1] == -(-V // 32),
+              "mask: int32 [M, ceil(V / 32)]")
+        masks = mask.shape[0]
+        _need(mask.shape[1] == 1 or mask.stride(1) == 1, "the rows of mask must be contiguous")
+        ld_mask = mask.stride(0) if masks > 1 else mask.shape[1]
+        _need(ld_mask >= mask.shape[1], "rows that overlap")
+        _need(mask_index is not None or masks in (1, B), "mask: one row, or B, or a mask_index")
+    if mask_index is not None:
+        _need(mask is not None, "mask_index without a mask")
+        _ints("mask_index", mask_index, B)
+    if B:
+        _launch("vk_penalize_logits", device, _p(logits), _p(out), _DTYPES[logits.dtype], ld, ld_out, B, V,
+                _p(history) if T else None, _p(history_lens), T, ld_history, _p(repetition), _p(presence), _p(frequency), _p(bias),
+                ld_bias, _p(mask), ld_mask, masks, _p(mask_index))
+    return out
