@@ -25,7 +25,6 @@ struct Args {
   float* lse;                  // [B, H] or NULL
   int64_t stride_q, stride_kb, stride_ks, stride_pp, stride_table;
   int B, H, HK, P, S, n_pages, page_shift, max_pages;
-  float scale;
 };
 
 // Reports group offsets that do not ascend from 0 to at most B.  Spread over the threads of the grid.
@@ -37,58 +36,461 @@ VK_DEV void check_offsets(const Args& a) {
   }
 }
 
-// One warp per (row, query head), one position at a time: the plain restatement of the formula.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) rows_kernel(Args a) {
-  constexpr int PER = D / 32;
-  const int lane = threadIdx.x & 31;
+constexpr int kThreads = 128;  // 4 warps
+constexpr int kStages = 3;     // of each warp's own ring
+
+// Work of one launch: prefix items (tile of rows, KV head, chunk) first, then tail items (row, KV head, tile of heads, chunk).
+// Partial results go to slot [split][b * H + h], prefix chunks first.
+struct Plan {
+  int prefix_tiles;   // at most; group g's tiles begin at floor(offset_g * r / rows) + g
+  int prefix_splits, prefix_chunk;
+  int tail_tiles;     // tiles of 16 heads of one (row, KV head)
+  int tail_splits, tail_chunk;
+  int prefix_items, tail_items;
+  float scale_log2;
+  float* ws_o;        // [prefix_splits + tail_splits][B * H][D]
+  float2* ws_ml;      // [prefix_splits + tail_splits][B * H]: maximum (of scores in base 2) and sum
+};
+
+template <typename T>
+VK_DEV void mma_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <>
+VK_DEV void mma_16816<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  mma_bf16_16816(d, a, b0, b1);
+}
+template <>
+VK_DEV void mma_16816<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two probabilities rounded to the type, and in *sum the sum of what they became.
+template <typename T>
+VK_DEV uint32_t pack_p(float x, float y, float* sum);
+template <>
+VK_DEV uint32_t pack_p<__nv_bfloat16>(float x, float y, float* sum) {
+  const uint32_t u = pack_bf16x2(x, y);
+  *sum += bf16_lo(u) + bf16_hi(u);
+  return u;
+}
+template <>
+VK_DEV uint32_t pack_p<__half>(float x, float y, float* sum) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  *sum += f.x + f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 bytes from global to shared memory, zeros where !use.
+VK_DEV void cp_async16(uint32_t dst, const void* src, bool use) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(use ? 16 : 0) : "memory");
+}
+VK_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+VK_DEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Positions a warp takes at a time: 4 KB of K and of V.
+template <int D>
+struct Tile {
+  static constexpr int kPos = 2048 / D;              // 32 or 16
+  static constexpr int kHalf = kPos * D * 2;         // bytes of K or V
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kWarp = kStages * kStage;
+  static constexpr int kSmem = 4 * kWarp;
+  // byte offset of 16-byte chunk c of position p; chunks of eight neighbouring positions lie in different banks
+  static VK_DEV uint32_t at(int p, int c) { return p * (D * 2) + ((c ^ (p & 7)) << 4); }
+};
+
+// Where the keys and values of an item come from.
+template <typename T>
+struct Source {
+  const T* k;
+  const T* v;
+  int64_t stride;          // of a position, in elements (prefix)
+  const int32_t* table;    // page ids (tail)
+  int64_t stride_page;
+  int page_shift, n_pages;
+};
+
+// Loads positions p .. p + kPos - 1 (those at or past end: zeros) into one stage.  page: this lane's page id, that of
+// position p + lane.
+template <typename T, int D, bool PAGED>
+VK_DEV void load_tile(const Source<T>& s, uint32_t stage, int p, int end, int page) {
+  constexpr int kChunks = D / 8, kRows = 32 / kChunks, kLoads = Tile<D>::kPos / kRows;
+  const int lane = threadIdx.x & 31, c = lane % kChunks, r0 = lane / kChunks;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = r0 + i * kRows, pos = p + r;
+    int64_t off;
+    if (PAGED) {
+      const int pg = __shfl_sync(0xffffffffu, page, r);
+      off = pg * s.stride_page + static_cast<int64_t>(pos & ((1 << s.page_shift) - 1)) * s.stride;
+    } else {
+      off = pos * s.stride;
+    }
+    const bool use = pos < end;
+    off = use ? off + c * 8 : 0;
+    cp_async16(stage + Tile<D>::at(r, c), s.k + off, use);
+    cp_async16(stage + Tile<D>::kHalf + Tile<D>::at(r, c), s.v + off, use);
+  }
+}
+
+// The page of position pos, 0 (and a report) where the table names none.
+template <typename T>
+VK_DEV int page_at(const Source<T>& s, int pos, int end) {
+  if (pos >= end) return 0;
+  const int pg = s.table[pos >> s.page_shift];
+  if (pg >= 0 && pg < s.n_pages) return pg;
+  raise_error(ERR_BOUNDS);
+  return 0;
+}
+
+// Online softmax of 16 * MT rows (a row is one query head of one token) over the tiles first, first + step, ... of the
+// positions begin .. end - 1; q: the rows' operand fragments.  The warp's ring: kStages stages at `ring`.
+//
+// Scores, probabilities and the result stay in registers (m16n8k16: the accumulator of the first product is the operand of
+// the second); a tile is bound by its 8 KB from HBM, which kStages - 1 tiles of every warp in flight keep coming.
+template <typename T, int D, int MT, bool PAGED>
+VK_DEV void attend(const Source<T>& s, uint32_t ring, int begin, int end, int first, int step, float scale_log2,
+                   const uint32_t (&q)[MT][D / 16][4], float (&o)[MT][D / 8][4], float (&m)[MT][2], float (&l)[MT][2]) {
+  constexpr int kPos = Tile<D>::kPos, kN = kPos / 8;
+  const int lane = threadIdx.x & 31, t4 = lane & 3, j = lane >> 3, rr = lane & 7;
+#pragma unroll
+  for (int a = 0; a < MT; ++a) {
+    m[a][0] = m[a][1] = -INFINITY;
+    l[a][0] = l[a][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[a][i][0] = o[a][i][1] = o[a][i][2] = o[a][i][3] = 0.f;
+  }
+  const int tiles = (end - begin + kPos - 1) / kPos;
+  const int own_pos = lane % kPos;  // (16 positions: the upper lanes repeat the lower ones)
+  int page = 0, next = first;
+  if (PAGED) page = page_at(s, begin + next * kPos + own_pos, end);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (next < tiles) {
+      load_tile<T, D, PAGED>(s, ring + i * Tile<D>::kStage, begin + next * kPos, end, page);
+      next += step;
+      if (PAGED) page = page_at(s, begin + next * kPos + own_pos, end);
+    }
+    cp_async_commit();
+  }
+  int stage = 0;
+  for (int t = first; t < tiles; t += step) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    {
+      const int to = stage == 0 ? kStages - 1 : stage - 1;  // the stage that was read last
+      if (next < tiles) {
+        load_tile<T, D, PAGED>(s, ring + to * Tile<D>::kStage, begin + next * kPos, end, page);
+        next += step;
+        if (PAGED) page = page_at(s, begin + next * kPos + own_pos, end);
+      }
+      cp_async_commit();
+    }
+    const uint32_t kb = ring + stage * Tile<D>::kStage, vb = kb + Tile<D>::kHalf;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    // ---- S = Q K^T ----
+    float sc[MT][kN][4];
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) sc[a][n][0] = sc[a][n][1] = sc[a][n][2] = sc[a][n][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int n = 0; n < kN; n += 2) {
+        uint32_t b[4];
+        ldsm_x4(kb + Tile<D>::at(n * 8 + (j >> 1) * 8 + rr, ks * 2 + (j & 1)), b[0], b[1], b[2], b[3]);
+#pragma unroll
+        for (int a = 0; a < MT; ++a) {
+          mma_16816<T>(sc[a][n], q[a][ks], b[0], b[1]);
+          mma_16816<T>(sc[a][n + 1], q[a][ks], b[2], b[3]);
+        }
+      }
+    // ---- softmax in base 2; the sum is that of the rounded probabilities, which the product below uses ----
+    const int p0 = begin + t * kPos;
+    const bool partial = p0 + kPos > end;
+    uint32_t pr[MT][kN][2];
+#pragma unroll
+    for (int a = 0; a < MT; ++a) {
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[a][n][e] *= scale_log2;
+          if (partial && p0 + n * 8 + 2 * t4 + (e & 1) >= end) sc[a][n][e] = -INFINITY;
+        }
+        mx0 = fmaxf(mx0, fmaxf(sc[a][n][0], sc[a][n][1]));
+        mx1 = fmaxf(mx1, fmaxf(sc[a][n][2], sc[a][n][3]));
+      }
+#pragma unroll
+      for (int x = 1; x < 4; x <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+      }
+      const float mn0 = fmaxf(m[a][0], mx0), mn1 = fmaxf(m[a][1], mx1);
+      const float mu0 = mn0 == -INFINITY ? 0.f : mn0, mu1 = mn1 == -INFINITY ? 0.f : mn1;
+      const float f0 = fast_exp2(m[a][0] - mu0), f1 = fast_exp2(m[a][1] - mu1);
+      m[a][0] = mn0;
+      m[a][1] = mn1;
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        pr[a][n][0] = pack_p<T>(fast_exp2(sc[a][n][0] - mu0), fast_exp2(sc[a][n][1] - mu0), &s0);
+        pr[a][n][1] = pack_p<T>(fast_exp2(sc[a][n][2] - mu1), fast_exp2(sc[a][n][3] - mu1), &s1);
+      }
+      l[a][0] = l[a][0] * f0 + s0;
+      l[a][1] = l[a][1] * f1 + s1;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[a][i][0] *= f0;
+        o[a][i][1] *= f0;
+        o[a][i][2] *= f1;
+        o[a][i][3] *= f1;
+      }
+    }
+    // ---- O += P V ----
+#pragma unroll
+    for (int n = 0; n < kN; n += 2)
+#pragma unroll
+      for (int i = 0; i < D / 8; i += 2) {
+        uint32_t b[4];
+        ldsm_x4_t(vb + Tile<D>::at(n * 8 + (j & 1) * 8 + rr, i + (j >> 1)), b[0], b[1], b[2], b[3]);
+#pragma unroll
+        for (int a = 0; a < MT; ++a) {
+          const uint32_t pa[4] = {pr[a][n][0], pr[a][n][1], pr[a][n + 1][0], pr[a][n + 1][1]};
+          mma_16816<T>(o[a][i], pa, b[0], b[1]);
+          mma_16816<T>(o[a][i + 1], pa, b[2], b[3]);
+        }
+      }
+    __syncwarp();  // the stage may be loaded again
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int a = 0; a < MT; ++a)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int x = 1; x < 4; x <<= 1) l[a][e] += __shfl_xor_sync(0xffffffffu, l[a][e], x);
+}
+
+// Operand fragments of 16 * MT rows: row x is query head kvh * r + x % r of token b0 + x / r, x0 <= x < x1.
+template <typename T, int D, int MT>
+VK_DEV void load_q(const Args& a, int b0, int kvh, int r, int x0, int x1, uint32_t (&q)[MT][D / 16][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int x = x0 + i * 16 + e * 8 + g;
+      const bool use = x < x1;
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) +
+                                                            (use ? (b0 + x / r) * a.stride_q + (kvh * r + x % r) * D : 0));
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        q[i][ks][e] = use ? p[ks * 8 + t4] : 0u;
+        q[i][ks][e + 2] = use ? p[ks * 8 + t4 + 4] : 0u;
+      }
+    }
+}
+
+// Joins the WI warps of an item (through shared memory, which their rings have left) and writes the rows' partial results.
+template <int D, int MT, int WI>
+VK_DEV void store_partial(const Args& a, const Plan& pl, uint8_t* smem, int split, int b0, int kvh, int r, int x0, int x1,
+                          float (&o)[MT][D / 8][4], float (&m)[MT][2], float (&l)[MT][2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  const int64_t base = static_cast<int64_t>(split) * a.B * a.H;
+  if (WI == 1) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int x = x0 + i * 16 + e * 8 + g;
+        if (x >= x1) continue;
+        const int64_t row = base + static_cast<int64_t>(b0 + x / r) * a.H + kvh * r + x % r;
+        if (t4 == 0) pl.ws_ml[row] = make_float2(m[i][e], l[i][e]);
+        float* op = pl.ws_o + row * D + 2 * t4;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(op + d * 8) = make_float2(o[i][d][2 * e], o[i][d][2 * e + 1]);
+      }
+    return;
+  }
+  constexpr int kRows = 16 * MT;
+  float* so = reinterpret_cast<float*>(smem);                      // [4][kRows][D]
+  float2* sml = reinterpret_cast<float2*>(so + 4 * kRows * D);     // [4][kRows]
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int x = i * 16 + e * 8 + g;
+      if (t4 == 0) sml[warp * kRows + x] = make_float2(m[i][e], l[i][e]);
+      float* op = so + (warp * kRows + x) * D + 2 * t4;
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(op + d * 8) = make_float2(o[i][d][2 * e], o[i][d][2 * e + 1]);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
+    const int x = i / (D / 4), d = i % (D / 4) * 4;
+    if (x0 + x >= x1) break;
+    float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, sml[w * kRows + x].x);
+    float4 ot = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float mu = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 ml = sml[w * kRows + x];
+      const float f = fast_exp2(ml.x - mu);
+      const float4 v = *reinterpret_cast<const float4*>(so + (w * kRows + x) * D + d);
+      lt += f * ml.y;
+      ot.x += f * v.x;
+      ot.y += f * v.y;
+      ot.z += f * v.z;
+      ot.w += f * v.w;
+    }
+    const int64_t row = base + static_cast<int64_t>(b0 + (x0 + x) / r) * a.H + kvh * r + (x0 + x) % r;
+    if (d == 0) pl.ws_ml[row] = make_float2(mt, lt);
+    *reinterpret_cast<float4*>(pl.ws_o + row * D + d) = ot;
+  }
+}
+
+// An item without positions: sums of zero.
+VK_DEV void store_nothing(const Args& a, const Plan& pl, int split, int b0, int kvh, int r, int x0, int x1, int thread,
+                          int threads) {
+  for (int x = x0 + thread; x < x1; x += threads)
+    pl.ws_ml[(static_cast<int64_t>(split) * a.B + b0 + x / r) * a.H + kvh * r + x % r] = make_float2(-INFINITY, 0.f);
+}
+
+template <typename T, int D, int MT, int WI, bool PAGED>
+VK_DEV void run_item(const Args& a, const Plan& pl, uint8_t* smem, const Source<T>& s, int split, int begin, int end, int b0,
+                     int kvh, int r, int x0, int x1) {
+  const int warp = threadIdx.x >> 5;
+  if (begin >= end) {
+    if (WI == 1)
+      store_nothing(a, pl, split, b0, kvh, r, x0, x1, threadIdx.x & 31, 32);
+    else
+      store_nothing(a, pl, split, b0, kvh, r, x0, x1, threadIdx.x, kThreads);
+    return;
+  }
+  uint32_t q[MT][D / 16][4];
+  load_q<T, D, MT>(a, b0, kvh, r, x0, x1, q);
+  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  attend<T, D, MT, PAGED>(s, smem_u32(smem) + warp * Tile<D>::kWarp, begin, end, WI == 1 ? 0 : warp, WI, pl.scale_log2, q, o,
+                          m, l);
+  store_partial<D, MT, WI>(a, pl, smem, split, b0, kvh, r, x0, x1, o, m, l);
+}
+
+// MT: 16-row tiles of a prefix item.  WT: warps of a tail item.
+template <typename T, int D, int MT, int WT>
+__global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int found;
+  const int r = a.H / a.HK;
   pdl_wait();
   check_offsets(a);
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (item >= static_cast<int64_t>(a.B) * a.H) return;
-  const int b = static_cast<int>(item / a.H), h = static_cast<int>(item % a.H), kvh = h / (a.H / a.HK);
-  int g = 0;
-  while (g < a.P && a.offsets[g + 1] <= b) ++g;
-  if (g == a.P) return;  // behind the last group
-  const T* qp = static_cast<const T*>(a.q) + b * a.stride_q + h * D + lane * PER;
-  float q[PER], o[PER], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < PER; ++i) {
-    q[i] = to_f32<T>(qp[i]) * a.scale;
-    o[i] = 0.f;
+  if (static_cast<int>(blockIdx.x) < pl.prefix_items) {
+    constexpr int kRows = 16 * MT;
+    int item = blockIdx.x;
+    const int split = item % pl.prefix_splits;
+    item /= pl.prefix_splits;
+    const int kvh = item % a.HK, tile = item / a.HK;
+    // the group whose tiles hold this one: the last that begins at or before it
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    int n = 0;
+    for (int g = threadIdx.x; g < a.P; g += kThreads)
+      n += static_cast<int64_t>(a.offsets[g]) * r / kRows + g <= tile;
+    for (int x = 16; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&found, n);
+    __syncthreads();
+    const int g = found - 1;
+    if (g < 0) return;
+    const int b0 = a.offsets[g], b1 = min(a.offsets[g + 1], a.B);
+    if (b0 < 0 || b0 >= b1) return;
+    const int64_t x0 = (tile - static_cast<int64_t>(b0) * r / kRows - g) * kRows, all = static_cast<int64_t>(b1 - b0) * r;
+    if (x0 < 0 || x0 >= all) return;
+    const int x1 = static_cast<int>(x0 + kRows < all ? x0 + kRows : all);
+    Source<T> s{};
+    s.k = static_cast<const T*>(a.k_prefix) + g * a.stride_kb + kvh * D;
+    s.v = static_cast<const T*>(a.v_prefix) + g * a.stride_kb + kvh * D;
+    s.stride = a.stride_ks;
+    const int len = checked_len(a.prefix_lens[g], a.S), begin = split * pl.prefix_chunk;
+    run_item<T, D, MT, 4, false>(a, pl, smem, s, split, begin, min(begin + pl.prefix_chunk, len), b0, kvh, r,
+                                 static_cast<int>(x0), x1);
+    return;
   }
-  const int np = checked_len(a.prefix_lens[g], a.S);
-  const int nt = checked_len(a.tail_lens[b], a.max_pages << a.page_shift);
-  for (int j = 0; j < np + nt; ++j) {
-    int64_t off;
-    const T *kp, *vp;
-    if (j < np) {
-      off = g * a.stride_kb + j * a.stride_ks;
-      kp = static_cast<const T*>(a.k_prefix);
-      vp = static_cast<const T*>(a.v_prefix);
-    } else {
-      const int t = j - np;
-      int page = a.table[b * a.stride_table + (t >> a.page_shift)];
-      if (page < 0 || page >= a.n_pages) {
-        raise_error(ERR_BOUNDS);
-        page = 0;
-      }
-      off = page * a.stride_pp + static_cast<int64_t>(t & ((1 << a.page_shift) - 1)) * a.HK * D;
-      kp = static_cast<const T*>(a.k_pages);
-      vp = static_cast<const T*>(a.v_pages);
-    }
-    off += kvh * D + lane * PER;
-    float s = 0.f;
-    for (int i = 0; i < PER; ++i) s += q[i] * to_f32<T>(kp[off + i]);
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
-    const float f = expf(m - mu), p = expf(s - mu);
-    l = l * f + p;
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * f + p * to_f32<T>(vp[off + i]);
+  const int per = WT == 1 ? 4 : 1;  // items of a CTA
+  int item = (blockIdx.x - pl.prefix_items) * per + (WT == 1 ? threadIdx.x >> 5 : 0);
+  if (item >= pl.tail_items) return;
+  const int split = item % pl.tail_splits;
+  item /= pl.tail_splits;
+  const int tile = item % pl.tail_tiles;
+  item /= pl.tail_tiles;
+  const int kvh = item % a.HK, b = item / a.HK;
+  if (b >= a.offsets[a.P]) return;  // behind the last group
+  Source<T> s{};
+  s.k = static_cast<const T*>(a.k_pages) + kvh * D;
+  s.v = static_cast<const T*>(a.v_pages) + kvh * D;
+  s.stride = static_cast<int64_t>(a.HK) * D;
+  s.table = a.table + b * a.stride_table;
+  s.stride_page = a.stride_pp;
+  s.page_shift = a.page_shift;
+  s.n_pages = a.n_pages;
+  const int len = checked_len(a.tail_lens[b], a.max_pages << a.page_shift), begin = split * pl.tail_chunk;
+  run_item<T, D, 1, WT, true>(a, pl, smem, s, pl.prefix_splits + split, begin, min(begin + pl.tail_chunk, len), b, kvh, r,
+                              tile * 16, min(tile * 16 + 16, r));
+}
+
+// Joins the partial results of a row and head: W warps each take every W-th split, four in flight.
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(32 * W) join_kernel(Args a, Plan pl, int splits) {
+  constexpr int PER = D / 32;
+  __shared__ float so[W][D];
+  __shared__ float2 sml[W];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  const int64_t row = blockIdx.x, rows = static_cast<int64_t>(a.B) * a.H;
+  if (row / a.H >= a.offsets[a.P]) return;
+  float m = -INFINITY, l = 0.f, o[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = 0.f;
+  auto add = [&](float2 ml, const float* v) {
+    const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+    const float fa = fast_exp2(m - mu), fb = fast_exp2(ml.x - mu);
+    l = l * fa + ml.y * fb;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = o[i] * fa + v[i] * fb;
     m = mn;
+  };
+  for (int s = warp; s < splits; s += W) {
+    const float2 ml = pl.ws_ml[s * rows + row];
+    if (ml.y == 0.f) continue;  // nothing there: the values were not written
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = pl.ws_o[(s * rows + row) * D + lane * PER + i];
+    add(ml, v);
   }
-  T* op = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.H + h) * D + lane * PER;
-  for (int i = 0; i < PER; ++i) op[i] = from_f32<T>(l > 0.f ? o[i] / l : l);  // l NaN stays NaN, l 0 gives 0
-  if (a.lse && lane == 0) a.lse[static_cast<int64_t>(b) * a.H + h] = l > 0.f || l != l ? m + logf(l) : -INFINITY;
+  if (W > 1) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) so[warp][lane * PER + i] = o[i];
+    if (lane == 0) sml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp) return;
+    for (int w = 1; w < W; ++w)
+      if (sml[w].y != 0.f) add(sml[w], &so[w][lane * PER]);
+  }
+  T* op = static_cast<T*>(a.out) + row * D + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) op[i] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m * 0.69314718055994531f + logf(l);
 }
 
 }  // namespace sattn

@@ -883,9 +883,72 @@ int vk_scatter_embed(void* x, const int64_t* rows, int64_t n, int64_t x_rows, co
 }
 
 // ---- several candidates of a chunk ------------------------------------------------------------------------------
+}  // extern "C"
+
+namespace vk {
+// Splits of an axis of `most` positions among `items` independent pieces of work: as many as fill the resident CTAs (four per
+// SM) twice, chunks no shorter than `shortest` and no longer than 2048 positions.
+static int splits_of(int most, int64_t items, int shortest, int64_t ctas) {
+  if (most <= 0) return 0;
+  const int64_t want = (2 * ctas + items - 1) / items, top = (most + shortest - 1) / shortest, low = (most + 2047) / 2048;
+  return static_cast<int>(std::max(low, std::min(want, top)));
+}
+static int chunk_of(int most, int splits) { return splits ? ((most + splits - 1) / splits + 31) / 32 * 32 : 32; }
+
+struct SharedPlan {
+  int mt, wt;
+  sattn::Plan p;
+  int64_t prefix_items, tail_items;
+};
+static SharedPlan shared_plan(int B, int H, int HK, int D, int P, int S, int max_tail) {
+  SharedPlan r;
+  memset(&r, 0, sizeof(r));
+  const int64_t ratio = H / HK, ctas = 4 * 148;
+  r.mt = B * ratio > 16 * static_cast<int64_t>(P) ? 2 : 1;
+  const int64_t tiles = P + B * ratio / (16 * r.mt);
+  r.p.prefix_tiles = static_cast<int>(tiles);
+  r.p.prefix_splits = splits_of(S, tiles * HK, 128, ctas);
+  r.p.prefix_chunk = chunk_of(S, r.p.prefix_splits);
+  r.p.tail_tiles = static_cast<int>((ratio + 15) / 16);
+  const int64_t pieces = static_cast<int64_t>(B) * HK * r.p.tail_tiles;
+  r.wt = pieces >= 4 * ctas ? 1 : 4;
+  r.p.tail_splits = splits_of(max_tail, r.wt == 1 ? pieces / 4 : pieces, 128, ctas);
+  r.p.tail_chunk = chunk_of(max_tail, r.p.tail_splits);
+  r.prefix_items = tiles * HK * r.p.prefix_splits;
+  r.tail_items = pieces * r.p.tail_splits;
+  return r;
+}
+
+template <typename T, int D, int MT, int WT>
+static int shared_split(const sattn::Args& a, const sattn::Plan& p, unsigned grid, void* stream) {
+  auto kern = sattn::split_kernel<T, D, MT, WT>;
+  const int smem = std::max(sattn::Tile<D>::kSmem, 4 * 16 * MT * (D + 2) * 4);
+  if (!ensure_smem(kern, smem)) return VK_ERR_CUDA;
+  return launch(kern, dim3(grid), dim3(sattn::kThreads), smem, stream, 1, a, p);
+}
+
+template <typename T, int D>
+static int shared_run(const sattn::Args& a, const SharedPlan& r, void* stream) {
+  const int64_t grid = r.prefix_items + (r.wt == 1 ? (r.tail_items + 3) / 4 : r.tail_items);
+  if (grid >= (int64_t(1) << 31) || r.tail_items >= (int64_t(1) << 31)) return VK_ERR_ARG;
+  const unsigned n = static_cast<unsigned>(grid);
+  const int rc = r.mt == 1 ? (r.wt == 1 ? shared_split<T, D, 1, 1>(a, r.p, n, stream) : shared_split<T, D, 1, 4>(a, r.p, n, stream))
+                           : (r.wt == 1 ? shared_split<T, D, 2, 1>(a, r.p, n, stream) : shared_split<T, D, 2, 4>(a, r.p, n, stream));
+  if (rc != VK_OK) return rc;
+  const int splits = r.p.prefix_splits + r.p.tail_splits;
+  const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H);
+  return splits > 16 ? launch(sattn::join_kernel<T, D, 8>, dim3(rows), dim3(256), 0, stream, 1, a, r.p, splits)
+                     : launch(sattn::join_kernel<T, D, 1>, dim3(rows), dim3(32), 0, stream, 1, a, r.p, splits);
+}
+
+}  // namespace vk
+
+extern "C" {
+
 size_t vk_shared_attention_workspace_bytes(int B, int H, int HK, int D, int P, int S, int max_tail) {
-  if (B <= 0 || H <= 0 || HK <= 0 || D <= 0 || P <= 0 || S <= 0 || max_tail < 0) return 0;
-  return 16;
+  if (B <= 0 || H <= 0 || HK <= 0 || H % HK || D <= 0 || P <= 0 || S <= 0 || max_tail < 0) return 0;
+  const SharedPlan r = shared_plan(B, H, HK, D, P, S, max_tail);
+  return static_cast<size_t>(r.p.prefix_splits + r.p.tail_splits) * B * H * (D + 2) * 4;
 }
 
 int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* k_prefix, const void* v_prefix,
@@ -938,13 +1001,15 @@ int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* 
   a.n_pages = n_pages;
   a.page_shift = log2_of(page);
   a.max_pages = max_pages;
-  a.scale = scale;
-  void (*kern)(sattn::Args) = nullptr;
+  SharedPlan r = shared_plan(B, H, HK, D, P, S, max_pages * page);
+  r.p.prefix_items = static_cast<int>(r.prefix_items);
+  r.p.tail_items = static_cast<int>(r.tail_items);
+  r.p.scale_log2 = scale * 1.4426950408889634f;
+  r.p.ws_o = static_cast<float*>(workspace);
+  r.p.ws_ml = reinterpret_cast<float2*>(r.p.ws_o + static_cast<size_t>(r.p.prefix_splits + r.p.tail_splits) * B * H * D);
   if (dtype == VK_BF16)
-    kern = D == 64 ? sattn::rows_kernel<__nv_bfloat16, 64> : sattn::rows_kernel<__nv_bfloat16, 128>;
-  else
-    kern = D == 64 ? sattn::rows_kernel<__half, 64> : sattn::rows_kernel<__half, 128>;
-  return launch(kern, dim3(blocks_for(static_cast<int64_t>(B) * H, 4)), dim3(128), 0, stream, 1, a);
+    return D == 64 ? shared_run<__nv_bfloat16, 64>(a, r, stream) : shared_run<__nv_bfloat16, 128>(a, r, stream);
+  return D == 64 ? shared_run<__half, 64>(a, r, stream) : shared_run<__half, 128>(a, r, stream);
 }
 
 // Scratch of the page calls, one region after another: ints, then the moves.
