@@ -6,6 +6,8 @@
 // A row with nothing to attend gives 0 (lse -inf); rows behind the last group are not touched.
 #pragma once
 
+#include <type_traits>
+
 #include "vk_common.cuh"
 
 namespace vk {
@@ -44,12 +46,13 @@ constexpr int kStages = 3;     // of each warp's own ring
 struct Plan {
   int prefix_tiles;   // at most; group g's tiles begin at floor(offset_g * r / rows) + g
   int prefix_splits, prefix_chunk;
+  int prefix_slots;   // partial results of a row's prefix: its splits, or two for each split of wide_kernel
   int tail_tiles;     // tiles of 16 heads of one (row, KV head)
   int tail_splits, tail_chunk;
   int prefix_items, tail_items;
   float scale_log2;
-  float* ws_o;        // [prefix_splits + tail_splits][B * H][D]
-  float2* ws_ml;      // [prefix_splits + tail_splits][B * H]: maximum (of scores in base 2) and sum
+  float* ws_o;        // [prefix_slots + tail_splits][B * H][D]
+  float2* ws_ml;      // [prefix_slots + tail_splits][B * H]: maximum (of scores in base 2) and sum
 };
 
 template <typename T>
@@ -388,6 +391,40 @@ VK_DEV void run_item(const Args& a, const Plan& pl, uint8_t* smem, const Source<
   store_partial<D, MT, WI>(a, pl, smem, split, b0, kvh, r, x0, x1, o, m, l);
 }
 
+// The rows of a prefix item: rows x0 .. x1 - 1 (numbered as in load_q) of the group g; x0 >= x1: none.
+struct Rows {
+  int g, b0, kvh, split, x0, x1;
+};
+// The item of this CTA of `threads` threads with tiles of kRows rows.  found: one shared word.
+template <int kRows, int threads>
+VK_DEV Rows find_rows(const Args& a, const Plan& pl, int* found) {
+  const int r = a.H / a.HK;
+  Rows w{};
+  int item = blockIdx.x;
+  w.split = item % pl.prefix_splits;
+  item /= pl.prefix_splits;
+  w.kvh = item % a.HK;
+  const int tile = item / a.HK;
+  // the group whose tiles hold this one: the last that begins at or before it
+  if (threadIdx.x == 0) *found = 0;
+  __syncthreads();
+  int n = 0;
+  for (int g = threadIdx.x; g < a.P; g += threads) n += static_cast<int64_t>(a.offsets[g]) * r / kRows + g <= tile;
+  for (int x = 16; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
+  if ((threadIdx.x & 31) == 0) atomicAdd(found, n);
+  __syncthreads();
+  w.g = *found - 1;
+  if (w.g < 0) return w;
+  w.b0 = a.offsets[w.g];
+  const int b1 = min(a.offsets[w.g + 1], a.B);
+  if (w.b0 < 0 || w.b0 >= b1) return w;
+  const int64_t x0 = (tile - static_cast<int64_t>(w.b0) * r / kRows - w.g) * kRows, all = static_cast<int64_t>(b1 - w.b0) * r;
+  if (x0 < 0 || x0 >= all) return w;
+  w.x0 = static_cast<int>(x0);
+  w.x1 = static_cast<int>(x0 + kRows < all ? x0 + kRows : all);
+  return w;
+}
+
 // MT: 16-row tiles of a prefix item.  WT: warps of a tail item.
 template <typename T, int D, int MT, int WT>
 __global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
@@ -397,34 +434,14 @@ __global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
   pdl_wait();
   check_offsets(a);
   if (static_cast<int>(blockIdx.x) < pl.prefix_items) {
-    constexpr int kRows = 16 * MT;
-    int item = blockIdx.x;
-    const int split = item % pl.prefix_splits;
-    item /= pl.prefix_splits;
-    const int kvh = item % a.HK, tile = item / a.HK;
-    // the group whose tiles hold this one: the last that begins at or before it
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
-    int n = 0;
-    for (int g = threadIdx.x; g < a.P; g += kThreads)
-      n += static_cast<int64_t>(a.offsets[g]) * r / kRows + g <= tile;
-    for (int x = 16; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
-    if ((threadIdx.x & 31) == 0) atomicAdd(&found, n);
-    __syncthreads();
-    const int g = found - 1;
-    if (g < 0) return;
-    const int b0 = a.offsets[g], b1 = min(a.offsets[g + 1], a.B);
-    if (b0 < 0 || b0 >= b1) return;
-    const int64_t x0 = (tile - static_cast<int64_t>(b0) * r / kRows - g) * kRows, all = static_cast<int64_t>(b1 - b0) * r;
-    if (x0 < 0 || x0 >= all) return;
-    const int x1 = static_cast<int>(x0 + kRows < all ? x0 + kRows : all);
+    const Rows w = find_rows<16 * MT, kThreads>(a, pl, &found);
+    if (w.x0 >= w.x1) return;
     Source<T> s{};
-    s.k = static_cast<const T*>(a.k_prefix) + g * a.stride_kb + kvh * D;
-    s.v = static_cast<const T*>(a.v_prefix) + g * a.stride_kb + kvh * D;
+    s.k = static_cast<const T*>(a.k_prefix) + w.g * a.stride_kb + w.kvh * D;
+    s.v = static_cast<const T*>(a.v_prefix) + w.g * a.stride_kb + w.kvh * D;
     s.stride = a.stride_ks;
-    const int len = checked_len(a.prefix_lens[g], a.S), begin = split * pl.prefix_chunk;
-    run_item<T, D, MT, 4, false>(a, pl, smem, s, split, begin, min(begin + pl.prefix_chunk, len), b0, kvh, r,
-                                 static_cast<int>(x0), x1);
+    const int len = checked_len(a.prefix_lens[w.g], a.S), begin = w.split * pl.prefix_chunk;
+    run_item<T, D, MT, 4, false>(a, pl, smem, s, w.split, begin, min(begin + pl.prefix_chunk, len), w.b0, w.kvh, r, w.x0, w.x1);
     return;
   }
   const int per = WT == 1 ? 4 : 1;  // items of a CTA
@@ -445,8 +462,331 @@ __global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
   s.page_shift = a.page_shift;
   s.n_pages = a.n_pages;
   const int len = checked_len(a.tail_lens[b], a.max_pages << a.page_shift), begin = split * pl.tail_chunk;
-  run_item<T, D, 1, WT, true>(a, pl, smem, s, pl.prefix_splits + split, begin, min(begin + pl.tail_chunk, len), b, kvh, r,
+  run_item<T, D, 1, WT, true>(a, pl, smem, s, pl.prefix_slots + split, begin, min(begin + pl.tail_chunk, len), b, kvh, r,
                               tile * 16, min(tile * 16 + 16, r));
+}
+
+// ---- wide groups -------------------------------------------------------------------------------------------------
+// Prefix attention of up to 256 rows of one group and KV head on the 5th-generation tensor cores, one CTA per SM:
+//   warp 0      TMA: 128-position tiles of K and V, one after another, into a ring of units
+//   warp 1      MMA issue (one lane); two streams s = 0, 1, each with its own 128 x 128 scores and 128 x D result in TMEM:
+//                 S_s = Q K_j^T, then, once the softmax has put P over S_s, O_s += P V_j
+//   warps 2-5   softmax of stream 0, one row per thread; warps 6-9 of stream 1
+// More than 128 rows: the streams are the two halves of the rows and share every tile.  Otherwise they take the even and the
+// odd tiles for the same rows and give two partial results.  While one stream's softmax runs, the tensor cores work for the
+// other.  S_s(j + 1) is issued behind O_s(j), so a completed S_s also says that the last product has left P and O.
+template <int D>
+struct Wide {
+  static constexpr int kThreads = 320;
+  static constexpr int kPos = 128;
+  static constexpr int kUnit = kPos * D * 2;            // bytes of a K or V tile, and of a Q tile
+  static constexpr int kUnits = D == 128 ? 5 : 8;
+  static constexpr int kRing = 2 * kUnit;               // behind the two Q tiles
+  static constexpr int kBars = kRing + kUnits * kUnit;
+  static constexpr int kSmem = kBars + 256 + 1024;
+  static constexpr uint32_t kColO = 256;                // S_0, S_1 at 0 and 128; O_0, O_1 at kColO and kColO + D
+  static constexpr uint32_t kCols = 512;
+};
+
+// MN-major operand of a [positions][D] tile stored as D / 64 sub-tiles of 128 positions x 128 bytes (128-byte swizzle).
+VK_DEV uint64_t sdesc_v(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(16384u >> 4) << 16;   // next 64 columns: the next sub-tile
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;    // next 8 positions
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;            // SWIZZLE_128B
+  return d;
+}
+
+template <typename T>
+VK_DEV uint32_t pack2(float x, float y);
+template <>
+VK_DEV uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  return pack_bf16x2(x, y);
+}
+template <>
+VK_DEV uint32_t pack2<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Wide<D>::kThreads, 1)
+    wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Args a, Plan pl) {
+  using W = Wide<D>;
+  constexpr uint32_t kF16 = sizeof(T) == 2 && std::is_same<T, __half>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + W::kBars);
+  uint64_t* u_full = q_full + 1;
+  uint64_t* u_empty = u_full + W::kUnits;
+  uint64_t* s_full = u_empty + W::kUnits;  // [2] scores in TMEM
+  uint64_t* p_full = s_full + 2;           // [2] probabilities in TMEM, result rescaled
+  uint64_t* o_full = p_full + 2;           // [2] last product done
+  uint64_t* tmem_free = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_free + 1);
+  int* found = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = a.H / a.HK;
+
+  pdl_wait();
+  check_offsets(a);
+  const Rows w = find_rows<2 * W::kPos, W::kThreads>(a, pl, found);
+  if (w.x0 >= w.x1) return;
+  const int n_rows = w.x1 - w.x0;
+  const bool both = n_rows > W::kPos;  // the streams share the tiles
+  const int len = checked_len(a.prefix_lens[w.g], a.S), begin = w.split * pl.prefix_chunk;
+  const int end = min(begin + pl.prefix_chunk, len);
+  if (begin >= end) {
+    store_nothing(a, pl, 2 * w.split, w.b0, w.kvh, r, w.x0, w.x1, threadIdx.x, W::kThreads);
+    store_nothing(a, pl, 2 * w.split + 1, w.b0, w.kvh, r, w.x0, w.x1, threadIdx.x, W::kThreads);
+    return;
+  }
+  const int tiles = (end - begin + W::kPos - 1) / W::kPos;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 8);
+    for (int i = 0; i < W::kUnits; ++i) {
+      mbar_init(&u_full[i], 1);
+      mbar_init(&u_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(tmem_free, 8);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, W::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      for (int u = 0; u < 2 * tiles; ++u) {
+        const int slot = u % W::kUnits;
+        if (u >= W::kUnits && !mbar_wait(&u_empty[slot], ((u / W::kUnits) & 1) ^ 1)) {
+          raise_error(ERR_WAIT_EMPTY);
+          break;
+        }
+        uint8_t* to = smem + W::kRing + slot * W::kUnit;
+        const CUtensorMap* map = u & 1 ? &tmV : &tmK;
+        mbar_expect_tx(&u_full[slot], W::kUnit);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(to + c * 16384, map, &u_full[slot], c * 64, w.kvh, begin + (u >> 1) * W::kPos, w.g);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issue ----------------
+    constexpr uint32_t kTypes = kF16 ? (1u << 7) | (1u << 10) : 0u;  // fp16 operands: clear the bf16 format bits
+    constexpr uint32_t idesc_s = idesc_bf16_f32(W::kPos, W::kPos) & ~kTypes;
+    constexpr uint32_t idesc_o = (idesc_bf16_f32(W::kPos, D) & ~kTypes) | (1u << 16);  // V is MN-major
+    bool ok = mbar_wait(q_full, 0);
+    tc_fence_after();
+    auto wait_unit = [&](int u) { ok = ok && mbar_wait(&u_full[u % W::kUnits], (u / W::kUnits) & 1); };
+    auto release = [&](int u) {
+      if (ok && lane == 0) umma_commit(&u_empty[u % W::kUnits]);
+    };
+    auto scores = [&](int s, int j) {
+      wait_unit(2 * j);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok || lane != 0) return;
+      tc_fence_after();
+      const uint32_t qb = smem_u32(smem + (both ? s : 0) * W::kUnit);
+      const uint32_t kb = smem_u32(smem + W::kRing + (2 * j) % W::kUnits * W::kUnit);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks)
+        umma_bf16(tmem + s * 128, sdesc_k_sw128(qb + ks / 4 * 16384) + 2 * (ks % 4), sdesc_k_sw128(kb + ks / 4 * 16384) + 2 * (ks % 4),
+                  idesc_s, ks != 0);
+      umma_commit(&s_full[s]);
+    };
+    auto product = [&](int s, int j, int c, bool last) {  // c: how many came before in this stream
+      wait_unit(2 * j + 1);
+      const uint32_t vb = smem_u32(smem + W::kRing + (2 * j + 1) % W::kUnits * W::kUnit);
+      const int rows = end - begin - j * W::kPos;
+      if (rows < W::kPos && (s == 0 || !both)) {  // what lies behind the prefix may hold anything: 0 * NaN is NaN
+        for (int i = lane; i < (W::kPos - rows) * (D / 8); i += 32) {
+          const int pos = rows + i / (D / 8), ch = i % (D / 8);
+          *reinterpret_cast<uint4*>(smem + W::kRing + (2 * j + 1) % W::kUnits * W::kUnit + ch / 8 * 16384 + pos * 128 +
+                                    ch % 8 * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+      }
+      ok = ok && mbar_wait(&p_full[s], c & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok || lane != 0) return;
+      tc_fence_after();
+#pragma unroll
+      for (int ks = 0; ks < W::kPos / 16; ++ks)
+        umma_bf16_tmem_a(tmem + W::kColO + s * D, tmem + s * 128 + ks * 8, sdesc_v(vb + ks * 2048), idesc_o, (c | ks) != 0);
+      if (last) umma_commit(&o_full[s]);
+    };
+    if (both) {
+      scores(0, 0);
+      scores(1, 0);
+      release(0);
+      for (int j = 0; j < tiles && ok; ++j) {
+        const bool last = j == tiles - 1;
+        product(0, j, j, last);
+        if (!last) scores(0, j + 1);
+        product(1, j, j, last);
+        release(2 * j + 1);
+        if (!last) {
+          scores(1, j + 1);
+          release(2 * j + 2);
+        }
+      }
+    } else {
+      scores(0, 0);
+      release(0);
+      if (tiles > 1) {
+        scores(1, 1);
+        release(2);
+      }
+      for (int j = 0; j < tiles && ok; ++j) {
+        product(j & 1, j, j >> 1, j + 2 >= tiles);
+        release(2 * j + 1);
+        if (j + 2 < tiles) {
+          scores(j & 1, j + 2);
+          release(2 * j + 4);
+        }
+      }
+    }
+    if (!ok && lane == 0) raise_error(ERR_WAIT_FULL);
+  } else {
+    // ---------------- softmax ----------------
+    const int s = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int x = w.x0 + (both ? s * W::kPos : 0) + row;  // this thread's row of the group
+    const bool used = x < w.x1;
+    const int h = w.kvh * r + x % r;
+    // Q: thread row s of stream s's tile (one tile: the streams load a half of the columns each)
+    {
+      const T* qp = static_cast<const T*>(a.q) + (used ? (w.b0 + x / r) * a.stride_q + h * D : 0);
+      uint8_t* to = smem + (both ? s : 0) * W::kUnit + row * 128;
+      const int c0 = both ? 0 : s * (D / 16), c1 = both ? D / 8 : c0 + D / 16;
+      for (int c = c0; c < c1; ++c) {
+        const uint4 v = used ? *reinterpret_cast<const uint4*>(qp + c * 8) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(to + c / 8 * 16384 + (((c & 7) ^ (row & 7)) << 4)) = v;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t ts = tmem + s * 128 + lanes, to = tmem + W::kColO + s * D + lanes;
+    const int mine = both ? tiles : (tiles + 1 - s) / 2;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int c = 0; c < mine; ++c) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], c & 1));
+      if (!ok) break;
+      tc_fence_after();
+      float v[W::kPos];
+#pragma unroll
+      for (int i = 0; i < W::kPos; i += 16) tmem_ld16(ts + i, v + i);
+      tmem_wait_ld();
+      const int left = end - begin - (both ? c : 2 * c + s) * W::kPos;
+      if (left < W::kPos) {
+#pragma unroll
+        for (int i = 0; i < W::kPos; ++i)
+          if (i >= left) v[i] = -INFINITY;
+      }
+      float mx8[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx8[k] = v[k];
+#pragma unroll
+      for (int i = 8; i < W::kPos; i += 8)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], v[i + k]);
+      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) * pl.scale_log2;
+      // the reference maximum follows only when it is passed by more than 2^8: probabilities up to 256 round as well
+      const float m_new = mx > m + 8.f || m == -INFINITY ? fmaxf(m, mx) : m;
+      const float mu = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = fast_exp2(m - mu);
+      const float2 sc2 = make_float2(pl.scale_log2, pl.scale_log2), nm2 = make_float2(-mu, -mu);
+      float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int c0 = 0; c0 < W::kPos; c0 += 32) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 t = __ffma2_rn(make_float2(v[c0 + i], v[c0 + i + 1]), sc2, nm2);
+          const float2 p = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+          rs4[(i >> 1) & 3] = __fadd2_rn(rs4[(i >> 1) & 3], p);
+          pk[i / 2] = pack2<T>(p.x, p.y);
+        }
+        tmem_st16(ts + c0 / 2, pk);
+      }
+      const float2 rs2 = __fadd2_rn(__fadd2_rn(rs4[0], rs4[1]), __fadd2_rn(rs4[2], rs4[3]));
+      if (c > 0 && !__all_sync(0xffffffffu, alpha == 1.f)) {
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          float o[32];
+          uint32_t ob[32];
+          tmem_ld16(to + c0, o);
+          tmem_ld16(to + c0 + 16, o + 16);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(o[i] * alpha);
+          tmem_st16(to + c0, ob);
+          tmem_st16(to + c0 + 16, ob + 16);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[s]);
+      l = alpha * l + rs2.x + rs2.y;
+      m = m_new;
+    }
+    if (mine > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[s], 0));
+    if (!ok && lane == 0) raise_error(ERR_WAIT_ACCUM);
+    if (ok) {
+      tc_fence_after();
+      const int64_t at = static_cast<int64_t>(w.b0 + x / r) * a.H + h, rows = static_cast<int64_t>(a.B) * a.H;
+      const int64_t slot = (2 * w.split + (both ? 0 : s)) * rows + at;
+      if (mine > 0) {
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          float o[32];
+          tmem_ld16(to + c0, o);
+          tmem_ld16(to + c0 + 16, o + 16);
+          tmem_wait_ld();
+          if (used) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(pl.ws_o + slot * D + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      }
+      if (used) {
+        pl.ws_ml[slot] = make_float2(m, l);
+        if (both) pl.ws_ml[slot + rows] = make_float2(-INFINITY, 0.f);
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(tmem_free);
+  }
+  if (warp == 1) {
+    if (!mbar_wait(tmem_free, 0) && lane == 0) raise_error(ERR_WAIT_ACCUM);
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, W::kCols);
+  }
 }
 
 // Joins the partial results of a row and head: W warps each take every W-th split, four in flight.

@@ -2,6 +2,7 @@
 // headers are included here so that all kernels share one device error word without relocatable device code.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 #include <utility>
 
 #include "decode_attention.cuh"
@@ -895,7 +896,24 @@ static int splits_of(int most, int64_t items, int shortest, int64_t ctas) {
 }
 static int chunk_of(int most, int splits) { return splits ? ((most + splits - 1) / splits + 31) / 32 * 32 : 32; }
 
+// Splits of wide_kernel's prefixes: the number that finishes first on `sms` CTAs at a time, counted in tiles of 128 positions;
+// an item costs three more than its tiles (pipeline fill, partial results).
+static int wide_splits(int64_t items, int S, int sms) {
+  const int64_t tiles = (S + 127) / 128;
+  int64_t best = 0;
+  int at = 1;
+  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
+    const int64_t cost = (items * s + sms - 1) / sms * ((tiles + s - 1) / s + 3);
+    if (s == 1 || cost < best) {
+      best = cost;
+      at = static_cast<int>(s);
+    }
+  }
+  return at;
+}
+
 struct SharedPlan {
+  bool wide;
   int mt, wt;
   sattn::Plan p;
   int64_t prefix_items, tail_items;
@@ -903,18 +921,26 @@ struct SharedPlan {
 static SharedPlan shared_plan(int B, int H, int HK, int D, int P, int S, int max_tail) {
   SharedPlan r;
   memset(&r, 0, sizeof(r));
-  const int64_t ratio = H / HK, ctas = 4 * 148;
-  r.mt = B * ratio > 16 * static_cast<int64_t>(P) ? 2 : 1;
-  const int64_t tiles = P + B * ratio / (16 * r.mt);
-  r.p.prefix_tiles = static_cast<int>(tiles);
-  r.p.prefix_splits = splits_of(S, tiles * HK, 128, ctas);
-  r.p.prefix_chunk = chunk_of(S, r.p.prefix_splits);
+  const int64_t ratio = H / HK, rows = B * ratio, ctas = 4 * 148;
+  r.wide = rows > 32 * static_cast<int64_t>(P);
+  if (r.wide) {
+    r.p.prefix_tiles = static_cast<int>(P + rows / 256);
+    r.p.prefix_splits = wide_splits(std::max<int64_t>(P, (rows + 255) / 256) * HK, S, 148);
+    r.p.prefix_chunk = ((S + r.p.prefix_splits - 1) / r.p.prefix_splits + 127) / 128 * 128;
+    r.p.prefix_slots = 2 * r.p.prefix_splits;
+  } else {
+    r.mt = rows > 16 * static_cast<int64_t>(P) ? 2 : 1;
+    r.p.prefix_tiles = static_cast<int>(P + rows / (16 * r.mt));
+    r.p.prefix_splits = splits_of(S, static_cast<int64_t>(r.p.prefix_tiles) * HK, 128, ctas);
+    r.p.prefix_chunk = chunk_of(S, r.p.prefix_splits);
+    r.p.prefix_slots = r.p.prefix_splits;
+  }
   r.p.tail_tiles = static_cast<int>((ratio + 15) / 16);
   const int64_t pieces = static_cast<int64_t>(B) * HK * r.p.tail_tiles;
   r.wt = pieces >= 4 * ctas ? 1 : 4;
   r.p.tail_splits = splits_of(max_tail, r.wt == 1 ? pieces / 4 : pieces, 128, ctas);
   r.p.tail_chunk = chunk_of(max_tail, r.p.tail_splits);
-  r.prefix_items = tiles * HK * r.p.prefix_splits;
+  r.prefix_items = static_cast<int64_t>(r.p.prefix_tiles) * HK * r.p.prefix_splits;
   r.tail_items = pieces * r.p.tail_splits;
   return r;
 }
@@ -928,14 +954,31 @@ static int shared_split(const sattn::Args& a, const sattn::Plan& p, unsigned gri
 }
 
 template <typename T, int D>
-static int shared_run(const sattn::Args& a, const SharedPlan& r, void* stream) {
-  const int64_t grid = r.prefix_items + (r.wt == 1 ? (r.tail_items + 3) / 4 : r.tail_items);
-  if (grid >= (int64_t(1) << 31) || r.tail_items >= (int64_t(1) << 31)) return VK_ERR_ARG;
-  const unsigned n = static_cast<unsigned>(grid);
-  const int rc = r.mt == 1 ? (r.wt == 1 ? shared_split<T, D, 1, 1>(a, r.p, n, stream) : shared_split<T, D, 1, 4>(a, r.p, n, stream))
-                           : (r.wt == 1 ? shared_split<T, D, 2, 1>(a, r.p, n, stream) : shared_split<T, D, 2, 4>(a, r.p, n, stream));
+static int shared_run(const sattn::Args& a, SharedPlan r, void* stream) {
+  const int64_t tails = r.wt == 1 ? (r.tail_items + 3) / 4 : r.tail_items;
+  if (r.prefix_items + tails >= (int64_t(1) << 31) || r.tail_items >= (int64_t(1) << 31)) return VK_ERR_ARG;
+  int rc = VK_OK;
+  if (r.wide) {
+    CUtensorMap mk, mv;
+    const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const uint64_t dims[4] = {D, static_cast<uint64_t>(a.HK), static_cast<uint64_t>(a.S), static_cast<uint64_t>(a.P)};
+    const uint64_t strides[3] = {D * 2, static_cast<uint64_t>(a.stride_ks) * 2, static_cast<uint64_t>(a.stride_kb) * 2};
+    const uint32_t box[4] = {64, 1, 128, 1};
+    if (!make_map(&mk, type, a.k_prefix, 4, dims, strides, box, true) || !make_map(&mv, type, a.v_prefix, 4, dims, strides, box, true))
+      return VK_ERR_ARG;
+    auto kern = sattn::wide_kernel<T, D>;
+    if (!ensure_smem(kern, sattn::Wide<D>::kSmem)) return VK_ERR_CUDA;
+    rc = launch(kern, dim3(static_cast<unsigned>(r.prefix_items)), dim3(sattn::Wide<D>::kThreads), sattn::Wide<D>::kSmem, stream, 1,
+                mk, mv, a, r.p);
+    r.prefix_items = 0;
+  }
+  r.p.prefix_items = static_cast<int>(r.prefix_items);
+  const unsigned n = static_cast<unsigned>(r.prefix_items + tails);
+  if (rc == VK_OK && n)
+    rc = r.mt == 2 ? (r.wt == 1 ? shared_split<T, D, 2, 1>(a, r.p, n, stream) : shared_split<T, D, 2, 4>(a, r.p, n, stream))
+                   : (r.wt == 1 ? shared_split<T, D, 1, 1>(a, r.p, n, stream) : shared_split<T, D, 1, 4>(a, r.p, n, stream));
   if (rc != VK_OK) return rc;
-  const int splits = r.p.prefix_splits + r.p.tail_splits;
+  const int splits = r.p.prefix_slots + r.p.tail_splits;
   const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H);
   return splits > 16 ? launch(sattn::join_kernel<T, D, 8>, dim3(rows), dim3(256), 0, stream, 1, a, r.p, splits)
                      : launch(sattn::join_kernel<T, D, 1>, dim3(rows), dim3(32), 0, stream, 1, a, r.p, splits);
@@ -948,7 +991,7 @@ extern "C" {
 size_t vk_shared_attention_workspace_bytes(int B, int H, int HK, int D, int P, int S, int max_tail) {
   if (B <= 0 || H <= 0 || HK <= 0 || H % HK || D <= 0 || P <= 0 || S <= 0 || max_tail < 0) return 0;
   const SharedPlan r = shared_plan(B, H, HK, D, P, S, max_tail);
-  return static_cast<size_t>(r.p.prefix_splits + r.p.tail_splits) * B * H * (D + 2) * 4;
+  return static_cast<size_t>(r.p.prefix_slots + r.p.tail_splits) * B * H * (D + 2) * 4;
 }
 
 int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* k_prefix, const void* v_prefix,
@@ -1002,11 +1045,10 @@ int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* 
   a.page_shift = log2_of(page);
   a.max_pages = max_pages;
   SharedPlan r = shared_plan(B, H, HK, D, P, S, max_pages * page);
-  r.p.prefix_items = static_cast<int>(r.prefix_items);
   r.p.tail_items = static_cast<int>(r.tail_items);
   r.p.scale_log2 = scale * 1.4426950408889634f;
   r.p.ws_o = static_cast<float*>(workspace);
-  r.p.ws_ml = reinterpret_cast<float2*>(r.p.ws_o + static_cast<size_t>(r.p.prefix_splits + r.p.tail_splits) * B * H * D);
+  r.p.ws_ml = reinterpret_cast<float2*>(r.p.ws_o + static_cast<size_t>(r.p.prefix_slots + r.p.tail_splits) * B * H * D);
   if (dtype == VK_BF16)
     return D == 64 ? shared_run<__nv_bfloat16, 64>(a, r, stream) : shared_run<__nv_bfloat16, 128>(a, r, stream);
   return D == 64 ? shared_run<__half, 64>(a, r, stream) : shared_run<__half, 128>(a, r, stream);
