@@ -106,6 +106,17 @@ def test_penalize_logits_refuses(change):
     assert "CUDA" not in str(e.value)
 
 
+def test_penalize_logits_refuses_overlapping_out():
+    a = {k: v for k, v in _good_penal().items() if k not in ("logits",)}
+    wide = torch.zeros(4, 100)
+    for x, out in ((wide[:3, :40], wide[:3, 20:60]), (wide[:3, :40], wide[1:, :40]), (wide[:3, 60:], wide[:3, 99:].as_strided((3, 40), (100, 1)))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.penalize_logits(x, out=out, **a)
+    for x, out in ((wide[:3, :40], wide[:3, 50:90]), (wide[:3, 50:90], wide[:3, :40]), (wide[:3, :40], wide[:3, :40])):
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.penalize_logits(x, out=out, **a)
+
+
 def test_entry_points_refuse():
     lib = _lib.load()
     ARG, NO = _lib.VK_ERR_ARG, _lib.VK_ERR_UNSUPPORTED

@@ -984,6 +984,32 @@ static int shared_run(const sattn::Args& a, SharedPlan r, void* stream) {
                      : launch(sattn::join_kernel<T, D, 1>, dim3(rows), dim3(32), 0, stream, 1, a, r.p, splits);
 }
 
+template <typename T, int VEC>
+static int penalize_launch(logit::Args a, void* stream) {
+  constexpr int kStep = logit::kThreads * VEC;
+  // the longest slice whose counters fit, or shorter ones where those would leave SMs idle (three CTAs each)
+  a.wide = a.T > 65535;
+  int64_t slice = logit::kMostSmem / (a.wide ? 4 : 2);
+  while (slice > kStep && static_cast<int64_t>(a.B) * ((a.V + slice - 1) / slice) < 3 * 148) slice = std::max<int64_t>(slice / 2, kStep);
+  const int64_t need = static_cast<int64_t>(a.V) + VEC - 1;
+  slice = std::min<int64_t>(slice, (need + kStep - 1) / kStep * kStep);
+  a.slice = static_cast<int>(slice);
+  a.slices = static_cast<int>((need + slice - 1) / slice);
+  const int64_t ctas = static_cast<int64_t>(a.slices) * a.B;
+  if (ctas >= (int64_t(1) << 31)) return VK_ERR_ARG;
+  auto kern = logit::penalize_kernel<T, VEC>;
+  const int64_t smem = (a.history ? slice * (a.wide ? 4 : 2) : 0) + slice / 8;
+  if (!ensure_smem(kern, logit::kMostSmem + logit::kMostSmem / 16)) return VK_ERR_CUDA;
+  return launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(logit::kThreads), smem, stream, 1, a);
+}
+
+template <typename T>
+static int penalize_run(const logit::Args& a, void* stream) {
+  const uintptr_t off = reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.out);
+  if (off % 16 || (a.B > 1 && (a.ld - a.ld_out) * static_cast<int64_t>(sizeof(T)) % 16)) return penalize_launch<T, 1>(a, stream);
+  return penalize_launch<T, 16 / sizeof(T)>(a, stream);
+}
+
 }  // namespace vk
 
 extern "C" {
@@ -1069,6 +1095,8 @@ static bool pool_ok(const int32_t* table, const int32_t* refs, int rows, int max
          static_cast<int64_t>(rows) * max_pages < (int64_t(1) << 31) &&
          static_cast<int64_t>(max_pages) * page < (int64_t(1) << 31);
 }
+// Grid of 256-thread CTAs over `cells`, one cell per thread while that fills the SMs less than eight times over.
+static unsigned cells_grid(int64_t cells) { return static_cast<unsigned>(std::min<int64_t>((cells + 255) / 256, 8 * 148)); }
 static pages::Pool pool_of(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page) {
   return pages::Pool{table, lens, refs, rows, max_pages, n_pages, log2_of(page)};
 }
@@ -1078,7 +1106,7 @@ int vk_pages_extend(int32_t* table, int32_t* lens, int32_t* refs, int rows, int 
                     size_t workspace_bytes, void* stream) {
   if (n == 0) return VK_OK;
   if (!pool_ok(table, refs, rows, max_pages, n_pages, page) || !lens || n < 0 || (!list && n != rows) || count <= 0 ||
-      count > max_pages * page || !page_out || !slot_out || !workspace || !aligned16(workspace) ||
+      count > max_pages * page || static_cast<int64_t>(n) * count >= (int64_t(1) << 31) || !page_out || !slot_out || !workspace || !aligned16(workspace) ||
       workspace_bytes < vk_pages_workspace_bytes(rows, max_pages, n_pages, n))
     return VK_ERR_ARG;
   pages::ExtendArgs a;
@@ -1090,17 +1118,29 @@ int vk_pages_extend(int32_t* table, int32_t* lens, int32_t* refs, int rows, int 
   a.slot = slot_out;
   a.claim = static_cast<int32_t*>(workspace);
   a.first = a.claim + rows;
-  a.free_list = a.first + n;
-  return launch(pages::extend_kernel, dim3(1), dim3(pages::kPlanThreads), 0, stream, 1, a);
+  a.len = a.first + n;
+  a.free_list = a.len + n;
+  const int64_t cells = static_cast<int64_t>(n) * count;
+  const bool few = cells <= pages::kFewCells;
+  const int rc = launch(pages::extend_kernel, dim3(1), dim3(pages::kPlanThreads), 0, stream, 1, a, few);
+  if (rc != VK_OK || few) return rc;
+  return launch(pages::extend_cells_kernel, dim3(cells_grid(cells)), dim3(256), 0, stream, 1, a);
 }
 
-static int copy_pages(const pages::CopyArgs& c, int64_t most, void* stream) {
+}  // extern "C"
+
+namespace vk {
+template <typename Also>
+static int copy_pages(const pages::CopyArgs& c, int64_t most, const Also& also, void* stream) {
   const int sms = device_sm_count();
   if (sms <= 0) return VK_ERR_CUDA;
   const int64_t units = most * c.layers * 2;
-  return launch(pages::copy_kernel, dim3(static_cast<unsigned>(units < 8 * sms ? units : 8 * sms)),
-                dim3(pages::kCopyThreads), 0, stream, 1, c);
+  return launch(pages::copy_kernel<Also>, dim3(static_cast<unsigned>(units < 8 * sms ? units : 8 * sms)),
+                dim3(pages::kCopyThreads), 0, stream, 1, c, also);
 }
+}  // namespace vk
+
+extern "C" {
 
 int vk_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page,
                   const int32_t* src, const int32_t* dst, int n, void* k, void* v, int layers, int token_bytes,
@@ -1122,7 +1162,10 @@ int vk_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int rows, int ma
   a.free_list = a.len + n;
   a.stage = a.free_list + n;
   a.moves = reinterpret_cast<pages::Move*>(static_cast<int32_t*>(workspace) + pages_ints(rows, max_pages, n_pages, n));
-  const int rc = launch(pages::fork_kernel, dim3(1), dim3(pages::kPlanThreads), 0, stream, 1, a);
+  const int64_t cells = static_cast<int64_t>(n) * max_pages;
+  const bool few = cells <= pages::kFewCells;
+  int rc = launch(pages::fork_kernel, dim3(1), dim3(pages::kPlanThreads), 0, stream, 1, a, few);
+  if (rc == VK_OK && !few) rc = launch(pages::fork_stage_kernel, dim3(cells_grid(cells)), dim3(256), 0, stream, 1, a);
   if (rc != VK_OK) return rc;
   pages::CopyArgs c;
   c.k = static_cast<uint8_t*>(k);
@@ -1134,7 +1177,7 @@ int vk_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int rows, int ma
   c.token_bytes = token_bytes;
   c.page_bytes = static_cast<int64_t>(token_bytes) * page;
   c.layer_bytes = c.page_bytes * n_pages;
-  return copy_pages(c, n, stream);
+  return few ? copy_pages(c, n, pages::JustCopy{}, stream) : copy_pages(c, n, pages::ForkWrite{a}, stream);
 }
 
 int vk_pages_free(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages,
@@ -1170,7 +1213,7 @@ int vk_pages_compact(int32_t* table, int32_t* refs, int rows, int max_pages, int
   c.token_bytes = token_bytes;
   c.page_bytes = static_cast<int64_t>(token_bytes) * page;
   c.layer_bytes = c.page_bytes * n_pages;
-  return copy_pages(c, n_pages / 2 + 1, stream);
+  return copy_pages(c, n_pages / 2 + 1, pages::Renumber{a.p, a.goes, a.counts + 1}, stream);
 }
 
 int vk_penalize_logits(const void* logits, void* out, int dtype, int64_t ld, int64_t ld_out, int B, int V,
@@ -1180,12 +1223,10 @@ int vk_penalize_logits(const void* logits, void* out, int dtype, int64_t ld, int
                        void* stream) {
   if (B == 0) return VK_OK;
   if (dtype < VK_BF16 || dtype > VK_F32) return VK_ERR_UNSUPPORTED;
-  if (B < 0 || V <= 0 || !logits || !out || ld < V || ld_out < V || (history && (!history_lens || T < 0 || ld_history < T)) ||
+  if (B < 0 || V <= 0 || V > 1 << 30 || !logits || !out || ld < V || ld_out < V || (history && (!history_lens || T < 0 || ld_history < T)) ||
       (bias && ld_bias != 0 && ld_bias < V))
     return VK_ERR_ARG;
   if (mask && (masks <= 0 || ld_mask < (V + 31) / 32 || (!mask_index && masks != 1 && masks != B))) return VK_ERR_ARG;
-  const int64_t slices = (V + logit::kSlice - 1) / logit::kSlice;
-  if (slices * B >= (int64_t(1) << 31)) return VK_ERR_ARG;
   logit::Args a;
   a.logits = logits;
   a.out = out;
@@ -1206,10 +1247,9 @@ int vk_penalize_logits(const void* logits, void* out, int dtype, int64_t ld, int
   a.B = B;
   a.V = V;
   a.T = T;
-  auto kern = dtype == VK_F32    ? logit::penalize_kernel<float>
-              : dtype == VK_BF16 ? logit::penalize_kernel<__nv_bfloat16>
-                                 : logit::penalize_kernel<__half>;
-  return launch(kern, dim3(static_cast<unsigned>(slices * B)), dim3(logit::kThreads), 0, stream, 1, a);
+  return dtype == VK_F32    ? penalize_run<float>(a, stream)
+         : dtype == VK_BF16 ? penalize_run<__nv_bfloat16>(a, stream)
+                            : penalize_run<__half>(a, stream);
 }
 
 // ---- host-side stitching (no device work) ------------------------------------------------------------------

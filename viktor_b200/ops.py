@@ -292,6 +292,7 @@ def scatter_embed(x, rows, emb, token):
 # ---------------------------------------------------------------- several candidates of a chunk (no reference counterpart)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _I32 = torch.int32
+_PAGES = (8, 16, 32, 64, 128, 256)
 
 
 def _launch(name, device, *args):
@@ -299,10 +300,10 @@ def _launch(name, device, *args):
     if device.type != "cuda":
         raise ValueError("viktor_b200 ops need CUDA tensors (there is no CPU path)")
     if device.index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream().cuda_stream)
+        call(name, *args, torch.cuda.current_stream(device).cuda_stream)
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch.cuda.current_stream().cuda_stream)
+            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 
 
 def _need(ok, what):
@@ -310,25 +311,29 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _same_device(*ts):
-    """The one device of the tensors."""
-    device = ts[0].device
+def _same_device(device, *ts):
     for t in ts:
-        _need(t is None or t.device == device, "all tensors must be on one device")
-    return device
+        if t is not None and t.device != device:
+            raise ValueError("all tensors must be on one device")
 
 
 def _ints(name, t, *shape):
-    _need(t.dtype == _I32 and tuple(t.shape) == shape and t.is_contiguous(), f"{name}: a contiguous int32 {list(shape)}")
+    if t.dtype != _I32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 {list(shape)}")
 
 
-def _cache_strides(t):
+def _cache_strides(shape, stride):
     """(row stride, position stride) in elements of [P, S, HK, D] whose positions are laid out as [HK, D]."""
-    P, S, HK, D = t.shape
-    sb, ss, sh, sd = t.stride()
+    P, S, HK, D = shape
+    sb, ss, sh, sd = stride
     _need(sd == 1 and (HK == 1 or sh == D), "the last two dimensions of a cache must be contiguous")
-    ss = ss if S > 1 else HK * D
-    return sb if P > 1 else ss * S, ss
+    if S == 1:
+        ss = HK * D
+    if P == 1:
+        sb = ss * S
+    _need(ss >= HK * D and sb >= ss * S and ss % 8 == 0 and sb % 8 == 0, "positions of a cache that overlap or are not 16-byte "
+          "aligned")
+    return sb, ss
 
 
 def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k_pages, v_pages, page_table, tail_lens,
@@ -344,55 +349,63 @@ def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k
     to attend gets 0 and -inf; rows behind the last group are not written.  What a cache holds behind a length is not
     used.  workspace: uint8, vk_shared_attention_workspace_bytes; calls that may run at the same time need one each (by
     default every call allocates its own)."""
-    _need(q.dim() == 3 and k_prefix.dim() == 4 and k_pages.dim() == 4, "q [B, H, D], caches of four dimensions")
-    B, H, D = q.shape
-    P, S, HK, _ = k_prefix.shape
-    n_pages, page = k_pages.shape[:2]
-    device = _same_device(q, k_prefix, v_prefix, prefix_lens, group_offsets, k_pages, v_pages, page_table, tail_lens, out,
-                          workspace)
-    dtype = q.dtype
-    _need(dtype in (torch.bfloat16, torch.float16) and k_prefix.dtype == v_prefix.dtype == k_pages.dtype == v_pages.dtype
-          == dtype, "q and the caches must all be bfloat16 or all float16")
-    _need(D in (64, 128), "head_dim must be 64 or 128")
+    q_shape, prefix_shape, pages_shape, table_shape = q.shape, k_prefix.shape, k_pages.shape, page_table.shape
+    _need(len(q_shape) == 3 and len(prefix_shape) == len(pages_shape) == 4 and len(table_shape) == 2,
+          "q [B, H, D], caches of four dimensions, page_table [B, max_pages]")
+    B, H, D = q_shape
+    P, S, HK, _ = prefix_shape
+    n_pages, page, _, _ = pages_shape
+    max_pages = table_shape[1]
+    device, dtype = q.device, q.dtype
+    _same_device(device, k_prefix, v_prefix, prefix_lens, group_offsets, k_pages, v_pages, page_table, tail_lens, out, workspace)
+    _need((dtype is torch.bfloat16 or dtype is torch.float16) and k_prefix.dtype is dtype and v_prefix.dtype is dtype
+          and k_pages.dtype is dtype and v_pages.dtype is dtype, "q and the caches must all be bfloat16 or all float16")
+    _need(D == 64 or D == 128, "head_dim must be 64 or 128")
     _need(P > 0 and S > 0 and HK > 0 and n_pages > 0 and H > 0 and H % HK == 0, "empty cache, or heads that do not divide")
-    _need(page in (8, 16, 32, 64, 128, 256), "pages hold a power of two from 8 to 256 tokens")
-    _need(k_prefix.shape == v_prefix.shape and k_prefix.shape[3] == D, "k_prefix and v_prefix: [P, S, HK, D]")
-    _need(k_pages.shape == v_pages.shape and k_pages.shape[2:] == (HK, D), "k_pages and v_pages: [n_pages, page, HK, D]")
-    _need(page_table.dim() == 2 and page_table.dtype == _I32 and page_table.shape[0] == B, "page_table: int32 [B, max_pages]")
-    max_pages = page_table.shape[1]
-    _need(max_pages < 2 or page_table.stride(1) == 1, "the rows of page_table must be contiguous")
-    stride_table = page_table.stride(0) if B > 1 else max_pages
-    _need(stride_table >= max_pages, "rows of page_table that overlap")
+    _need(page in _PAGES, "pages hold a power of two from 8 to 256 tokens")
+    _need(v_prefix.shape == prefix_shape and prefix_shape[3] == D, "k_prefix and v_prefix: [P, S, HK, D]")
+    _need(v_pages.shape == pages_shape and pages_shape[2] == HK and pages_shape[3] == D, "k_pages and v_pages: [n_pages, page, "
+          "HK, D]")
+    _need(page_table.dtype is _I32 and table_shape[0] == B, "page_table: int32 [B, max_pages]")
     _ints("prefix_lens", prefix_lens, P)
     _ints("group_offsets", group_offsets, P + 1)
     _ints("tail_lens", tail_lens, B)
-    stride_q = q.stride(0) if B > 1 else H * D
+    stride_table, one = page_table.stride()
+    if B <= 1:
+        stride_table = max_pages
+    _need((max_pages < 2 or one == 1) and stride_table >= max_pages, "the rows of page_table must be contiguous and must not "
+          "overlap")
+    stride_q, sh, one = q.stride()
+    if B <= 1:
+        stride_q = H * D
+    _need(one == 1 and (H == 1 or sh == D), "the heads of a row of q must be contiguous")
     _need(stride_q >= H * D and stride_q % 8 == 0, "the rows of q must be 16-byte aligned and must not overlap")
-    _need(q.stride(2) == 1 and (H == 1 or q.stride(1) == D), "the heads of a row of q must be contiguous")
-    kb, ks = _cache_strides(k_prefix)
-    _need((kb, ks) == _cache_strides(v_prefix), "k_prefix and v_prefix must have the same strides")
-    _need(ks >= HK * D and kb >= ks * S and ks % 8 == 0 and kb % 8 == 0, "positions of a cache that overlap or are not 16-byte "
-          "aligned")
-    pp, ps = _cache_strides(k_pages)
-    _need((pp, ps) == _cache_strides(v_pages) and ps == HK * D, "pages must be contiguous, with the same strides in k and v")
-    _need(pp >= page * ps and pp % 8 == 0, "pages that overlap or are not 16-byte aligned")
+    kb, ks = _cache_strides(prefix_shape, k_prefix.stride())
+    _need((kb, ks) == _cache_strides(prefix_shape, v_prefix.stride()), "k_prefix and v_prefix must have the same strides")
+    pp, ps = _cache_strides(pages_shape, k_pages.stride())
+    _need((pp, ps) == _cache_strides(pages_shape, v_pages.stride()) and ps == HK * D, "pages must be contiguous, with the same "
+          "strides in k and v")
     scale = D ** -0.5 if scale is None else float(scale)
     _need(0.0 < scale < float("inf"), "scale must be positive and finite")
+    q_at = q.data_ptr()
     if out is None:
-        out = torch.empty(B, H, D, dtype=dtype, device=device)
+        out = torch.empty(q_shape, dtype=dtype, device=device)
+        out_at = out.data_ptr()
     else:
-        _need(out.dtype == dtype and out.shape == q.shape and out.is_contiguous(), "out: contiguous, as q")
-        _need(B == 0 or out.data_ptr() + out.nbytes <= q.data_ptr() or out.data_ptr() >= q.data_ptr() + 2 * (
-            (B - 1) * stride_q + H * D), "out must not overlap q")
+        out_at = out.data_ptr()
+        _need(out.dtype is dtype and out.shape == q_shape and out.is_contiguous(), "out: contiguous, as q")
+        _need(B == 0 or out_at + 2 * B * H * D <= q_at or out_at >= q_at + 2 * ((B - 1) * stride_q + H * D), "out must not overlap q")
     lse = torch.empty(B, H, dtype=torch.float32, device=device) if return_lse else None
     if B:
         nbytes = load().vk_shared_attention_workspace_bytes(B, H, HK, D, P, S, max_pages * page)
         if workspace is None:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _need(workspace.is_contiguous() and workspace.nbytes >= nbytes, f"workspace: {nbytes} contiguous bytes")
-        _launch("vk_shared_attention", device, _p(q), stride_q, _DTYPES[dtype], _p(k_prefix), _p(v_prefix), _p(prefix_lens),
-                _p(group_offsets), P, S, kb, ks, _p(k_pages), _p(v_pages), n_pages, page, pp, _p(page_table), max_pages,
-                stride_table, _p(tail_lens), _p(out), _p(lse), B, H, HK, D, scale, _p(workspace), workspace.nbytes)
+        elif not workspace.is_contiguous() or workspace.nbytes < nbytes:
+            raise ValueError(f"workspace: {nbytes} contiguous bytes")
+        _launch("vk_shared_attention", device, q_at, stride_q, 0 if dtype is torch.bfloat16 else 1, k_prefix.data_ptr(),
+                v_prefix.data_ptr(), prefix_lens.data_ptr(), group_offsets.data_ptr(), P, S, kb, ks, k_pages.data_ptr(),
+                v_pages.data_ptr(), n_pages, page, pp, page_table.data_ptr(), max_pages, stride_table, tail_lens.data_ptr(), out_at,
+                _p(lse), B, H, HK, D, scale, workspace.data_ptr(), workspace.nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -408,13 +421,14 @@ class KVPages:
         self.layers, self.n_pages, self.page, hk, d = k.shape
         self.token_bytes = hk * d * k.element_size()
         _need(k.numel() > 0 and self.token_bytes % 16 == 0, "a token's K must be a multiple of 16 bytes")
-        _need(self.page in (8, 16, 32, 64, 128, 256), "pages hold a power of two from 8 to 256 tokens")
+        _need(self.page in _PAGES, "pages hold a power of two from 8 to 256 tokens")
         _need(table.dim() == 2 and table.numel() > 0, "table: int32 [rows, max_pages]")
         self.rows, self.max_pages = table.shape
         _ints("table", table, self.rows, self.max_pages)
         _ints("lens", lens, self.rows)
         _ints("refs", refs, self.n_pages)
-        self.device = _same_device(k, v, table, lens, refs)
+        self.device = k.device
+        _same_device(k.device, v, table, lens, refs)
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
 
     @classmethod
@@ -425,6 +439,12 @@ class KVPages:
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
                    torch.full((rows, max_pages), -1, **i32), torch.zeros(rows, **i32), torch.zeros(n_pages, **i32))
 
+    def _books(self):
+        return self.table.data_ptr(), self.lens.data_ptr(), self.refs.data_ptr(), self.rows, self.max_pages, self.n_pages
+
+    def _data(self):
+        return self.k.data_ptr(), self.v.data_ptr(), self.layers, self.token_bytes
+
     def _workspace(self, n):
         nbytes = load().vk_pages_workspace_bytes(self.rows, self.max_pages, self.n_pages, n)
         return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -433,9 +453,11 @@ class KVPages:
         """(pointer, count) of a list of rows; None stands for all of them."""
         if rows is None:
             return None, self.rows
-        _need(rows.dim() == 1 and rows.device == self.device, f"{name}: int32 [n] on the pages' device")
-        _ints(name, rows, rows.shape[0])
-        return rows.data_ptr(), rows.shape[0]
+        n = rows.numel()
+        _ints(name, rows, n)
+        if rows.device != self.device:
+            raise ValueError(f"{name}: on another device than the pages")
+        return rows.data_ptr(), n
 
 
 def pages_extend(pages: KVPages, count=1, rows=None):
@@ -448,8 +470,8 @@ def pages_extend(pages: KVPages, count=1, rows=None):
     page, slot = torch.empty(2, n, count, dtype=_I32, device=pages.device).unbind(0)
     if n:
         ws = pages._workspace(n)
-        _launch("vk_pages_extend", pages.device, _p(pages.table), _p(pages.lens), _p(pages.refs), pages.rows, pages.max_pages,
-                pages.n_pages, pages.page, ptr, n, count, _p(page), _p(slot), _p(ws), ws.nbytes)
+        _launch("vk_pages_extend", pages.device, *pages._books(), pages.page, ptr, n, count, page.data_ptr(), slot.data_ptr(),
+                ws.data_ptr(), ws.nbytes)
     return page, slot
 
 
@@ -462,17 +484,15 @@ def pages_fork(pages: KVPages, src, dst):
     _need(src is not None and dst is not None and n == m, "src and dst must have one length")
     if n:
         ws = pages._workspace(n)
-        _launch("vk_pages_fork", pages.device, _p(pages.table), _p(pages.lens), _p(pages.refs), pages.rows, pages.max_pages,
-                pages.n_pages, pages.page, src_ptr, dst_ptr, n, _p(pages.k), _p(pages.v), pages.layers, pages.token_bytes,
-                _p(ws), ws.nbytes)
+        _launch("vk_pages_fork", pages.device, *pages._books(), pages.page, src_ptr, dst_ptr, n, *pages._data(), ws.data_ptr(),
+                ws.nbytes)
 
 
 def pages_free(pages: KVPages, rows=None):
     """`rows` (int32 [n]; None: all) give their pages up and are empty."""
     ptr, n = pages._rows("rows", rows)
     if n:
-        _launch("vk_pages_free", pages.device, _p(pages.table), _p(pages.lens), _p(pages.refs), pages.rows, pages.max_pages,
-                pages.n_pages, ptr, n)
+        _launch("vk_pages_free", pages.device, *pages._books(), ptr, n)
 
 
 def pages_compact(pages: KVPages):
@@ -480,8 +500,9 @@ def pages_compact(pages: KVPages):
     ascending order.  Returns the count, int32 [1] on the device."""
     live = torch.empty(1, dtype=_I32, device=pages.device)
     ws = pages._workspace(0)
-    _launch("vk_pages_compact", pages.device, _p(pages.table), _p(pages.refs), pages.rows, pages.max_pages, pages.n_pages,
-            pages.page, _p(pages.k), _p(pages.v), pages.layers, pages.token_bytes, _p(live), _p(ws), ws.nbytes)
+    table, _, refs, rows, max_pages, n_pages = pages._books()
+    _launch("vk_pages_compact", pages.device, table, refs, rows, max_pages, n_pages, pages.page, *pages._data(), live.data_ptr(),
+            ws.data_ptr(), ws.nbytes)
     return live
 
 
@@ -496,46 +517,63 @@ def penalize_logits(logits, history=None, history_lens=None, repetition=None, pr
     and bias float32.  mask [M, ceil(V / 32)] int32: bit v % 32 of word v // 32 is 0 where v is forbidden, which gives -inf
     whatever the logit holds; mask_index [B] int32 names each row's mask (-1: none), without it M is B or 1.
     out: as logits (may be logits); returned."""
-    _need(logits.dim() == 2 and logits.dtype in _DTYPES, "logits: float32, bfloat16 or float16 [B, V]")
-    B, V = logits.shape
-    device = _same_device(logits, history, history_lens, repetition, presence, frequency, bias, mask, mask_index, out)
-    _need(V > 0 and (V == 1 or logits.stride(1) == 1), "the rows of logits must be contiguous")
+    shape, dtype, device = logits.shape, logits.dtype, logits.device
+    _need(len(shape) == 2 and dtype in _DTYPES, "logits: float32, bfloat16 or float16 [B, V]")
+    B, V = shape
+    _same_device(device, history, history_lens, repetition, presence, frequency, bias, mask, mask_index, out)
+    ld, one = logits.stride()
+    if B <= 1:
+        ld = V
+    _need(0 < V <= 1 << 30 and (V == 1 or one == 1) and ld >= V, "the rows of logits must be contiguous and must not overlap")
+    at = logits.data_ptr()
     if out is None:
-        out = torch.empty(B, V, dtype=logits.dtype, device=device)
-    _need(out.shape == logits.shape and out.dtype == logits.dtype and (V == 1 or out.stride(1) == 1), "out: as logits")
-    ld, ld_out = (t.stride(0) if B > 1 else V for t in (logits, out))
-    _need(ld_out >= V and ld >= V, "rows that overlap")
+        out = torch.empty(shape, dtype=dtype, device=device)
+        ld_out, out_at = V, out.data_ptr()
+    else:
+        ld_out, one = out.stride()
+        if B <= 1:
+            ld_out = V
+        out_at, size = out.data_ptr(), out.element_size()
+        _need(out.shape == shape and out.dtype is dtype and (V == 1 or one == 1) and ld_out >= V, "out: as logits")
+        if out_at != at or ld != ld_out:
+            # rows may lie side by side in one buffer, but not over one another
+            side = ld == ld_out and V * size <= (out_at - at) % (ld * size) <= (ld - V) * size
+            _need(side or out_at + ((B - 1) * ld_out + V) * size <= at or at + ((B - 1) * ld + V) * size <= out_at,
+                  "out must be logits or must not overlap it")
     T = ld_history = masks = ld_mask = ld_bias = 0
     if history is not None:
-        _need(history.dim() == 2 and history.shape[0] == B and history.dtype == torch.int64 and history_lens is not None,
+        _need(history.dim() == 2 and history.shape[0] == B and history.dtype is torch.int64 and history_lens is not None,
               "history: int64 [B, T], with history_lens")
         T = history.shape[1]
-        _need(T < 2 or history.stride(1) == 1, "the rows of history must be contiguous")
-        ld_history = history.stride(0) if B > 1 else T
-        _need(ld_history >= T, "rows that overlap")
+        ld_history, one = history.stride()
+        if B <= 1:
+            ld_history = T
+        _need((T < 2 or one == 1) and ld_history >= T, "the rows of history must be contiguous and must not overlap")
         _ints("history_lens", history_lens, B)
     else:
         _need(repetition is None and presence is None and frequency is None, "penalties need a history")
-    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        _need(t is None or (t.dtype == torch.float32 and t.shape == (B,) and t.is_contiguous()), f"{name}: float32 [B]")
+    for t in (repetition, presence, frequency):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != (B,) or not t.is_contiguous()):
+            raise ValueError("repetition, presence and frequency: contiguous float32 [B]")
     if bias is not None:
-        _need(bias.dtype == torch.float32 and bias.shape in ((V,), (B, V)) and (V == 1 or bias.stride(-1) == 1),
+        _need(bias.dtype is torch.float32 and (bias.shape == (V,) or bias.shape == shape) and (V == 1 or bias.stride(-1) == 1),
               "bias: float32 [V] or [B, V]")
         ld_bias = bias.stride(0) if bias.dim() == 2 and B > 1 else 0
-        _need(ld_bias == 0 or ld_bias >= V, "rows that overlap")
+        _need(ld_bias == 0 or ld_bias >= V, "rows of bias that overlap")
     if mask is not None:
-        _need(mask.dim() == 2 and mask.dtype == _I32 and mask.shape[0] > 0 and mask.shape[1] == -(-V // 32),
-              "mask: int32 [M, ceil(V / 32)]")
+        words = -(-V // 32)
+        _need(mask.dim() == 2 and mask.dtype is _I32 and mask.shape[0] > 0 and mask.shape[1] == words, "mask: int32 [M, ceil(V / 32)]")
         masks = mask.shape[0]
-        _need(mask.shape[1] == 1 or mask.stride(1) == 1, "the rows of mask must be contiguous")
-        ld_mask = mask.stride(0) if masks > 1 else mask.shape[1]
-        _need(ld_mask >= mask.shape[1], "rows that overlap")
+        ld_mask, one = mask.stride()
+        if masks == 1:
+            ld_mask = words
+        _need((words == 1 or one == 1) and ld_mask >= words, "the rows of mask must be contiguous and must not overlap")
         _need(mask_index is not None or masks in (1, B), "mask: one row, or B, or a mask_index")
     if mask_index is not None:
         _need(mask is not None, "mask_index without a mask")
         _ints("mask_index", mask_index, B)
     if B:
-        _launch("vk_penalize_logits", device, _p(logits), _p(out), _DTYPES[logits.dtype], ld, ld_out, B, V,
-                _p(history) if T else None, _p(history_lens), T, ld_history, _p(repetition), _p(presence), _p(frequency), _p(bias),
-                ld_bias, _p(mask), ld_mask, masks, _p(mask_index))
+        _launch("vk_penalize_logits", device, at, out_at, _DTYPES[dtype], ld, ld_out, B, V, _p(history) if T else None,
+                _p(history_lens), T, ld_history, _p(repetition), _p(presence), _p(frequency), _p(bias), ld_bias, _p(mask), ld_mask, masks,
+                _p(mask_index))
     return out
