@@ -46,13 +46,12 @@ constexpr int kStages = 3;     // of each warp's own ring
 struct Plan {
   int prefix_tiles;   // at most; group g's tiles begin at floor(offset_g * r / rows) + g
   int prefix_splits, prefix_chunk;
-  int prefix_slots;   // partial results of a row's prefix: its splits, or two for each split of wide_kernel
   int tail_tiles;     // tiles of 16 heads of one (row, KV head)
   int tail_splits, tail_chunk;
   int prefix_items, tail_items;
   float scale_log2;
-  float* ws_o;        // [prefix_slots + tail_splits][B * H][D]
-  float2* ws_ml;      // [prefix_slots + tail_splits][B * H]: maximum (of scores in base 2) and sum
+  float* ws_o;        // [prefix_splits + tail_splits][B * H][D]
+  float2* ws_ml;      // [prefix_splits + tail_splits][B * H]: maximum (of scores in base 2) and sum
 };
 
 template <typename T>
@@ -462,41 +461,41 @@ __global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
   s.page_shift = a.page_shift;
   s.n_pages = a.n_pages;
   const int len = checked_len(a.tail_lens[b], a.max_pages << a.page_shift), begin = split * pl.tail_chunk;
-  run_item<T, D, 1, WT, true>(a, pl, smem, s, pl.prefix_slots + split, begin, min(begin + pl.tail_chunk, len), b, kvh, r,
+  run_item<T, D, 1, WT, true>(a, pl, smem, s, pl.prefix_splits + split, begin, min(begin + pl.tail_chunk, len), b, kvh, r,
                               tile * 16, min(tile * 16 + 16, r));
 }
 
 // ---- wide groups -------------------------------------------------------------------------------------------------
 // Prefix attention of up to 256 rows of one group and KV head on the 5th-generation tensor cores, one CTA per SM:
-//   warp 0      TMA: 128-position tiles of K and V, one after another, into a ring of units
-//   warp 1      MMA issue (one lane); two streams s = 0, 1, each with its own 128 x 128 scores and 128 x D result in TMEM:
+//   warp 0      TMA: 64-position tiles of K and V, one after another, into a ring of units
+//   warp 1      MMA issue (one lane); two streams s = 0, 1, each with two 128 x 64 score buffers and a 128 x D result in TMEM:
 //                 S_s = Q K_j^T, then, once the softmax has put P over S_s, O_s += P V_j
 //   warps 2-5   softmax of stream 0, one row per thread; warps 6-9 of stream 1
 // More than 128 rows: the streams are the two halves of the rows and share every tile.  Otherwise they take the even and the
-// odd tiles for the same rows and give two partial results.  While one stream's softmax runs, the tensor cores work for the
-// other.  S_s(j + 1) is issued behind O_s(j), so a completed S_s also says that the last product has left P and O.
+// odd tiles for the same rows and are joined at the end.  A stream's next scores are ready while its softmax works: with one
+// buffer of 128 positions the softmax waited for the tensor cores half of the time (181 us against ... for 256 rows x 32 heads
+// on 32768 positions).
 template <int D>
 struct Wide {
   static constexpr int kThreads = 320;
-  static constexpr int kPos = 128;
-  static constexpr int kUnit = kPos * D * 2;            // bytes of a K or V tile, and of a Q tile
-  static constexpr int kUnits = D == 128 ? 5 : 8;
-  static constexpr int kRing = 2 * kUnit;               // behind the two Q tiles
+  static constexpr int kRows = 128;                     // of a stream
+  static constexpr int kPos = 64;
+  static constexpr int kUnit = kPos * D * 2;            // bytes of a K or V tile
+  static constexpr int kSub = kPos * 128;               // bytes of 64 of its columns
+  static constexpr int kQ = kRows * D * 2;              // bytes of a stream's queries
+  static constexpr int kUnits = D == 128 ? 10 : 16;
+  static constexpr int kRing = 2 * kQ;                  // behind the queries
   static constexpr int kBars = kRing + kUnits * kUnit;
-  static constexpr int kSmem = kBars + 256 + 1024;
-  static constexpr uint32_t kColO = 256;                // S_0, S_1 at 0 and 128; O_0, O_1 at kColO and kColO + D
+  static constexpr int kSmem = kBars + 512 + 1024;
+  static constexpr uint32_t kColO = 256;                // S_s: 128 s + 64 (tile & 1); O_s: kColO + D s
   static constexpr uint32_t kCols = 512;
 };
 
-// MN-major operand of a [positions][D] tile stored as D / 64 sub-tiles of 128 positions x 128 bytes (128-byte swizzle).
-VK_DEV uint64_t sdesc_v(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(16384u >> 4) << 16;   // next 64 columns: the next sub-tile
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;    // next 8 positions
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;            // SWIZZLE_128B
-  return d;
+// Shared-memory descriptor of a tile with rows of 128 bytes (128-byte swizzle, 8-row atoms 1024 bytes apart); across: bytes to
+// the next 64 columns of an MN-major operand.  Adding n to it moves it by 16 n bytes.
+VK_DEV uint64_t sdesc_tile(uint32_t saddr, uint32_t across) {
+  constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride, descriptor version, swizzle
+  return static_cast<uint64_t>(hi) << 32 | (saddr >> 4) | (across >> 4) << 16;
 }
 
 template <typename T>
@@ -521,26 +520,24 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + W::kBars);
   uint64_t* u_full = q_full + 1;
   uint64_t* u_empty = u_full + W::kUnits;
-  uint64_t* s_full = u_empty + W::kUnits;  // [2] scores in TMEM
-  uint64_t* p_full = s_full + 2;           // [2] probabilities in TMEM, result rescaled
-  uint64_t* o_full = p_full + 2;           // [2] last product done
-  uint64_t* tmem_free = o_full + 2;
+  uint64_t* s_full = u_empty + W::kUnits;  // [2][2] stream, buffer: scores in TMEM
+  uint64_t* p_full = s_full + 4;           // [2][2] probabilities in TMEM, result rescaled
+  uint64_t* o_full = p_full + 4;           // [2][2] stream, tile & 1: product done
+  uint64_t* tmem_free = o_full + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_free + 1);
   int* found = reinterpret_cast<int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int r = a.H / a.HK;
 
   pdl_wait();
   check_offsets(a);
-  const Rows w = find_rows<2 * W::kPos, W::kThreads>(a, pl, found);
+  const Rows w = find_rows<2 * W::kRows, W::kThreads>(a, pl, found);
   if (w.x0 >= w.x1) return;
-  const int n_rows = w.x1 - w.x0;
-  const bool both = n_rows > W::kPos;  // the streams share the tiles
+  const bool both = w.x1 - w.x0 > W::kRows;  // the streams share the tiles
   const int len = checked_len(a.prefix_lens[w.g], a.S), begin = w.split * pl.prefix_chunk;
   const int end = min(begin + pl.prefix_chunk, len);
   if (begin >= end) {
-    store_nothing(a, pl, 2 * w.split, w.b0, w.kvh, r, w.x0, w.x1, threadIdx.x, W::kThreads);
-    store_nothing(a, pl, 2 * w.split + 1, w.b0, w.kvh, r, w.x0, w.x1, threadIdx.x, W::kThreads);
+    store_nothing(a, pl, w.split, w.b0, w.kvh, r, w.x0, w.x1, threadIdx.x, W::kThreads);
     return;
   }
   const int tiles = (end - begin + W::kPos - 1) / W::kPos;
@@ -551,9 +548,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       mbar_init(&u_full[i], 1);
       mbar_init(&u_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 4);  // (one for each buffer: the softmax may be a tile ahead of the products)
       mbar_init(&o_full[i], 1);
     }
     mbar_init(tmem_free, 8);
@@ -584,97 +581,128 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         mbar_expect_tx(&u_full[slot], W::kUnit);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(to + c * 16384, map, &u_full[slot], c * 64, w.kvh, begin + (u >> 1) * W::kPos, w.g);
+          tma_load_4d(to + c * W::kSub, map, &u_full[slot], c * 64, w.kvh, begin + (u >> 1) * W::kPos, w.g);
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issue ----------------
+    // ---------------- MMA issue: the whole warp in step, one lane issues ----------------
     constexpr uint32_t kTypes = kF16 ? (1u << 7) | (1u << 10) : 0u;  // fp16 operands: clear the bf16 format bits
-    constexpr uint32_t idesc_s = idesc_bf16_f32(W::kPos, W::kPos) & ~kTypes;
-    constexpr uint32_t idesc_o = (idesc_bf16_f32(W::kPos, D) & ~kTypes) | (1u << 16);  // V is MN-major
-    bool ok = mbar_wait(q_full, 0);
-    tc_fence_after();
-    auto wait_unit = [&](int u) { ok = ok && mbar_wait(&u_full[u % W::kUnits], (u / W::kUnits) & 1); };
-    auto release = [&](int u) {
-      if (ok && lane == 0) umma_commit(&u_empty[u % W::kUnits]);
+    constexpr uint32_t idesc_s = idesc_bf16_f32(W::kRows, W::kPos) & ~kTypes;
+    constexpr uint32_t idesc_o = (idesc_bf16_f32(W::kRows, D) & ~kTypes) | (1u << 16);  // V is MN-major
+    const uint32_t one = elect_one();
+    const int n = __shfl_sync(0xffffffffu, tiles, 0), last = __shfl_sync(0xffffffffu, end - begin, 0) - (n - 1) * W::kPos;
+    const bool share = __shfl_sync(0xffffffffu, static_cast<int>(both), 0);
+    const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0), bars = base + W::kBars;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const auto at = [&](const uint64_t* bar0, int i) {  // shared address of a barrier
+      return bars + static_cast<uint32_t>(bar0 - q_full + i) * 8;
     };
-    auto scores = [&](int s, int j) {
-      wait_unit(2 * j);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok || lane != 0) return;
-      tc_fence_after();
-      const uint32_t qb = smem_u32(smem + (both ? s : 0) * W::kUnit);
-      const uint32_t kb = smem_u32(smem + W::kRing + (2 * j) % W::kUnits * W::kUnit);
+    bool late = !mbar_wait(q_full, 0);
+    const auto wait = [&](uint64_t* bar, uint32_t parity) { late |= !mbar_wait(bar, parity); };
+    // units of K are the even ones, of V the odd ones; kUnits is even
+    struct Cursor {
+      int slot;
+      uint32_t phase;
+      VK_DEV void next() {
+        slot += 2;
+        if (slot >= W::kUnits) {
+          slot -= W::kUnits;
+          phase ^= 1;
+        }
+      }
+    };
+    Cursor k{0, 0}, v{1, 0};
+    const auto scores = [&](int s, int c) {  // the c-th tile of stream s; its K is there
+      const uint64_t qd = sdesc_tile(base + (share ? s : 0) * W::kQ, 16);
+      const uint64_t kd = sdesc_tile(base + W::kRing + k.slot * W::kUnit, 16);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
-        umma_bf16(tmem + s * 128, sdesc_k_sw128(qb + ks / 4 * 16384) + 2 * (ks % 4), sdesc_k_sw128(kb + ks / 4 * 16384) + 2 * (ks % 4),
-                  idesc_s, ks != 0);
-      umma_commit(&s_full[s]);
+        umma_ss_if(one, tm + s * 128 + (c & 1) * 64, qd + ks / 4 * (16384 / 16) + 2 * (ks % 4), kd + ks / 4 * (W::kSub / 16) + 2 * (ks % 4),
+                   idesc_s, ks != 0);
+      umma_commit_if(one, at(s_full, 2 * s + (c & 1)));
     };
-    auto product = [&](int s, int j, int c, bool last) {  // c: how many came before in this stream
-      wait_unit(2 * j + 1);
-      const uint32_t vb = smem_u32(smem + W::kRing + (2 * j + 1) % W::kUnits * W::kUnit);
-      const int rows = end - begin - j * W::kPos;
-      if (rows < W::kPos && (s == 0 || !both)) {  // what lies behind the prefix may hold anything: 0 * NaN is NaN
-        for (int i = lane; i < (W::kPos - rows) * (D / 8); i += 32) {
-          const int pos = rows + i / (D / 8), ch = i % (D / 8);
-          *reinterpret_cast<uint4*>(smem + W::kRing + (2 * j + 1) % W::kUnits * W::kUnit + ch / 8 * 16384 + pos * 128 +
-                                    ch % 8 * 16) = make_uint4(0, 0, 0, 0);
+    const auto product = [&](int s, int c) {  // its V is there
+      wait(&p_full[2 * s + (c & 1)], (c >> 1) & 1);
+      tc_fence_after();
+      const uint64_t vd = sdesc_tile(base + W::kRing + v.slot * W::kUnit, W::kSub);
+#pragma unroll
+      for (int ks = 0; ks < W::kPos / 16; ++ks)
+        umma_ts_if(one, tm + W::kColO + s * D, tm + s * 128 + (c & 1) * 64 + ks * 8, vd + ks * (2048 / 16), idesc_o, (c | ks) != 0);
+      umma_commit_if(one, at(o_full, 2 * s + (c & 1)));
+    };
+    const auto wait_k = [&] {
+      wait(&u_full[k.slot], k.phase);
+      tc_fence_after();
+    };
+    const auto wait_v = [&](int j) {
+      wait(&u_full[v.slot], v.phase);
+      if (j == n - 1 && last < W::kPos) {  // what lies behind the prefix may hold anything, and 0 * NaN is NaN
+        for (int i = lane; i < (W::kPos - last) * (D / 8); i += 32) {
+          const int pos = last + i / (D / 8), ch = i % (D / 8);
+          *reinterpret_cast<uint4*>(smem + W::kRing + v.slot * W::kUnit + ch / 8 * W::kSub + pos * 128 + ch % 8 * 16) =
+              make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async();
         __syncwarp();
       }
-      ok = ok && mbar_wait(&p_full[s], c & 1);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok || lane != 0) return;
-      tc_fence_after();
-#pragma unroll
-      for (int ks = 0; ks < W::kPos / 16; ++ks)
-        umma_bf16_tmem_a(tmem + W::kColO + s * D, tmem + s * 128 + ks * 8, sdesc_v(vb + ks * 2048), idesc_o, (c | ks) != 0);
-      if (last) umma_commit(&o_full[s]);
     };
-    if (both) {
-      scores(0, 0);
-      scores(1, 0);
-      release(0);
-      for (int j = 0; j < tiles && ok; ++j) {
-        const bool last = j == tiles - 1;
-        product(0, j, j, last);
-        if (!last) scores(0, j + 1);
-        product(1, j, j, last);
-        release(2 * j + 1);
-        if (!last) {
-          scores(1, j + 1);
-          release(2 * j + 2);
+    const auto release = [&](Cursor& u) {
+      umma_commit_if(one, at(u_empty, u.slot));
+      u.next();
+    };
+    // scores run two tiles of a stream ahead of its products: into the buffer that the product before them has left
+    if (share) {
+      for (int j = 0; j < 2 && j < n; ++j) {
+        wait_k();
+        scores(0, j);
+        scores(1, j);
+        release(k);
+      }
+      for (int j = 0; j < n; ++j) {
+        const bool more = j + 2 < n;
+        wait_v(j);
+        product(0, j);
+        if (more) {
+          wait_k();
+          scores(0, j + 2);
         }
+        product(1, j);
+        release(v);
+        if (more) {
+          scores(1, j + 2);
+          release(k);
+        }
+        if (__any_sync(0xffffffffu, late)) break;
       }
     } else {
-      scores(0, 0);
-      release(0);
-      if (tiles > 1) {
-        scores(1, 1);
-        release(2);
+      for (int j = 0; j < 4 && j < n; ++j) {
+        wait_k();
+        scores(j & 1, j >> 1);
+        release(k);
       }
-      for (int j = 0; j < tiles && ok; ++j) {
-        product(j & 1, j, j >> 1, j + 2 >= tiles);
-        release(2 * j + 1);
-        if (j + 2 < tiles) {
-          scores(j & 1, j + 2);
-          release(2 * j + 4);
+      for (int j = 0; j < n; ++j) {
+        wait_v(j);
+        product(j & 1, j >> 1);
+        release(v);
+        if (j + 4 < n) {
+          wait_k();
+          scores(j & 1, (j >> 1) + 2);
+          release(k);
         }
+        if (__any_sync(0xffffffffu, late)) break;
       }
     }
-    if (!ok && lane == 0) raise_error(ERR_WAIT_FULL);
+    if (late) raise_error(ERR_WAIT_FULL);
   } else {
     // ---------------- softmax ----------------
     const int s = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const int x = w.x0 + (both ? s * W::kPos : 0) + row;  // this thread's row of the group
+    const int x = w.x0 + (both ? s * W::kRows : 0) + row;  // this thread's row of the group
     const bool used = x < w.x1;
     const int h = w.kvh * r + x % r;
-    // Q: thread row s of stream s's tile (one tile: the streams load a half of the columns each)
+    // Q: this thread's row of stream s's queries (queries of both: the streams load a half of the columns each)
     {
       const T* qp = static_cast<const T*>(a.q) + (used ? (w.b0 + x / r) * a.stride_q + h * D : 0);
-      uint8_t* to = smem + (both ? s : 0) * W::kUnit + row * 128;
+      uint8_t* to = smem + (both ? s : 0) * W::kQ + row * 128;
       const int c0 = both ? 0 : s * (D / 16), c1 = both ? D / 8 : c0 + D / 16;
       for (int c = c0; c < c1; ++c) {
         const uint4 v = used ? *reinterpret_cast<const uint4*>(qp + c * 8) : make_uint4(0, 0, 0, 0);
@@ -685,14 +713,18 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       if (lane == 0) mbar_arrive(q_full);
     }
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t ts = tmem + s * 128 + lanes, to = tmem + W::kColO + s * D + lanes;
+    const uint32_t to = tmem + W::kColO + s * D + lanes;
     const int mine = both ? tiles : (tiles + 1 - s) / 2;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+    // The product of the c-th tile is done.  Called when the scores of tile c or c + 1 are there, which were issued behind the
+    // product c - 2: of its barrier's phases only the one waited for can be open.
+    auto wait_product = [&](int c) { return __all_sync(0xffffffffu, mbar_wait(&o_full[2 * s + (c & 1)], (c >> 1) & 1)); };
     for (int c = 0; c < mine; ++c) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], c & 1));
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * s + (c & 1)], (c >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
+      const uint32_t ts = tmem + s * 128 + (c & 1) * 64 + lanes;
       float v[W::kPos];
 #pragma unroll
       for (int i = 0; i < W::kPos; i += 16) tmem_ld16(ts + i, v + i);
@@ -703,19 +735,15 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         for (int i = 0; i < W::kPos; ++i)
           if (i >= left) v[i] = -INFINITY;
       }
-      float mx8[8];
+      float mx4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mx8[k] = v[k];
+      for (int i = 4; i < W::kPos; i += 8)
 #pragma unroll
-      for (int i = 8; i < W::kPos; i += 8)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], v[i + k]);
-      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) * pl.scale_log2;
+        for (int k = 0; k < 4; ++k) mx4[k] = i + 4 < W::kPos ? fmaxf(fmaxf(mx4[k], v[i + k]), v[(i + 4 + k) % W::kPos]) : fmaxf(mx4[k], v[i + k]);
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * pl.scale_log2;
       // the reference maximum follows only when it is passed by more than 2^8: probabilities up to 256 round as well
       const float m_new = mx > m + 8.f || m == -INFINITY ? fmaxf(m, mx) : m;
       const float mu = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = fast_exp2(m - mu);
       const float2 sc2 = make_float2(pl.scale_log2, pl.scale_log2), nm2 = make_float2(-mu, -mu);
       float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -731,7 +759,11 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         tmem_st16(ts + c0 / 2, pk);
       }
       const float2 rs2 = __fadd2_rn(__fadd2_rn(rs4[0], rs4[1]), __fadd2_rn(rs4[2], rs4[3]));
+      const float alpha = fast_exp2(m - mu);
       if (c > 0 && !__all_sync(0xffffffffu, alpha == 1.f)) {
+        ok = wait_product(c - 1);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
         for (int c0 = 0; c0 < D; c0 += 32) {
           float o[32];
@@ -748,34 +780,61 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[s]);
+      if (lane == 0) mbar_arrive(&p_full[2 * s + (c & 1)]);
       l = alpha * l + rs2.x + rs2.y;
       m = m_new;
     }
-    if (mine > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[s], 0));
+    if (mine > 0 && ok) ok = wait_product(mine - 1);
     if (!ok && lane == 0) raise_error(ERR_WAIT_ACCUM);
-    if (ok) {
-      tc_fence_after();
-      const int64_t at = static_cast<int64_t>(w.b0 + x / r) * a.H + h, rows = static_cast<int64_t>(a.B) * a.H;
-      const int64_t slot = (2 * w.split + (both ? 0 : s)) * rows + at;
-      if (mine > 0) {
+    tc_fence_after();
+    // joined streams: stream 1 hands its result over in the queries' place (every product that reads them is done: its own, and
+    // those of stream 0 before stream 0 reads)
+    float* other = reinterpret_cast<float*>(smem);  // [D][128]
+    float2* other_ml = reinterpret_cast<float2*>(smem + W::kRing);  // [128], over the ring's first unit
+    if (!both) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (s == 1 && mine > 0) {
 #pragma unroll
         for (int c0 = 0; c0 < D; c0 += 32) {
           float o[32];
           tmem_ld16(to + c0, o);
           tmem_ld16(to + c0 + 16, o + 16);
           tmem_wait_ld();
-          if (used) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(pl.ws_o + slot * D + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          }
+          for (int i = 0; i < 32; ++i) other[(c0 + i) * 128 + row] = o[i];
         }
       }
-      if (used) {
-        pl.ws_ml[slot] = make_float2(m, l);
-        if (both) pl.ws_ml[slot + rows] = make_float2(-INFINITY, 0.f);
+      if (s == 1) other_ml[row] = make_float2(m, l);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if (both || s == 0) {
+      const int64_t slot = (static_cast<int64_t>(w.split) * a.B + w.b0 + x / r) * a.H + h;
+      float f0 = 1.f, f1 = 0.f;
+      if (!both && tiles > 1) {
+        const float2 ml = other_ml[row];
+        const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+        f0 = fast_exp2(m - mu);
+        f1 = fast_exp2(ml.x - mu);
+        l = l * f0 + ml.y * f1;
+        m = mn;
       }
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        float o[32];
+        tmem_ld16(to + c0, o);
+        tmem_ld16(to + c0 + 16, o + 16);
+        tmem_wait_ld();
+        if (!both && tiles > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + other[(c0 + i) * 128 + row] * f1;
+        }
+        if (used) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(pl.ws_o + slot * D + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      if (used) pl.ws_ml[slot] = make_float2(m, l);
     }
     tc_fence_before();
     __syncwarp();
@@ -789,47 +848,69 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   }
 }
 
-// Joins the partial results of a row and head: W warps each take every W-th split, four in flight.
+// Joins the partial results of a row and head: W warps each take every W-th run of 32 splits.  A warp's lanes take the weights of
+// 32 splits at once; then their values come four loads at a time.
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(32 * W) join_kernel(Args a, Plan pl, int splits) {
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) join_kernel(Args a, Plan pl, int splits) {
   constexpr int PER = D / 32;
-  __shared__ float so[W][D];
+  using V = typename std::conditional<PER == 2, float2, float4>::type;
+  __shared__ V so[W][32];
   __shared__ float2 sml[W];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
   pdl_wait();
-  const int64_t row = blockIdx.x, rows = static_cast<int64_t>(a.B) * a.H;
-  if (row / a.H >= a.offsets[a.P]) return;
+  pdl_launch_dependents();
+  const int64_t rows = static_cast<int64_t>(a.B) * a.H;
+  const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= rows || row / a.H >= a.offsets[a.P]) return;
   float m = -INFINITY, l = 0.f, o[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) o[i] = 0.f;
-  auto add = [&](float2 ml, const float* v) {
-    const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-    const float fa = fast_exp2(m - mu), fb = fast_exp2(ml.x - mu);
-    l = l * fa + ml.y * fb;
+  for (int s0 = warp * 32; s0 < splits; s0 += W * 32) {
+    const int n = min(32, splits - s0);
+    const float2 ml = lane < n ? pl.ws_ml[(s0 + lane) * rows + row] : make_float2(-INFINITY, 0.f);
+    float mn = ml.x;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * fa + v[i] * fb;
+    for (int x = 16; x > 0; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+    mn = fmaxf(mn, m);
+    const float mu = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - mu);
+    const float weight = ml.y == 0.f ? 0.f : fast_exp2(ml.x - mu);
+    l = l * f + ml.y * weight;  // this lane's share
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] *= f;
     m = mn;
-  };
-  for (int s = warp; s < splits; s += W) {
-    const float2 ml = pl.ws_ml[s * rows + row];
-    if (ml.y == 0.f) continue;  // nothing there: the values were not written
-    float v[PER];
+    const uint32_t there = __ballot_sync(0xffffffffu, ml.y != 0.f);  // (NaN too) elsewhere no values were written
+    const V* at = reinterpret_cast<const V*>(pl.ws_o + (s0 * rows + row) * D) + lane;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, weight, k);
+      if (!(there >> k & 1)) continue;
+      const V v = __ldcg(at + k * (rows * 32));
 #pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = pl.ws_o[(s * rows + row) * D + lane * PER + i];
-    add(ml, v);
+      for (int i = 0; i < PER; ++i) o[i] += wk * reinterpret_cast<const float*>(&v)[i];
+    }
   }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
   if (W > 1) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) so[warp][lane * PER + i] = o[i];
+    for (int i = 0; i < PER; ++i) reinterpret_cast<float*>(&so[warp][lane])[i] = o[i];
     if (lane == 0) sml[warp] = make_float2(m, l);
     __syncthreads();
     if (warp) return;
-    for (int w = 1; w < W; ++w)
-      if (sml[w].y != 0.f) add(sml[w], &so[w][lane * PER]);
+    for (int w = 1; w < W; ++w) {
+      const float2 ml = sml[w];
+      if (ml.y == 0.f) continue;
+      const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+      const float fa = fast_exp2(m - mu), fb = fast_exp2(ml.x - mu);
+      l = l * fa + ml.y * fb;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] = o[i] * fa + reinterpret_cast<const float*>(&so[w][lane])[i] * fb;
+      m = mn;
+    }
   }
   T* op = static_cast<T*>(a.out) + row * D + lane * PER;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) op[i] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+  for (int i = 0; i < PER; i += 2) *reinterpret_cast<uint32_t*>(op + i) = l == 0.f ? 0u : pack2<T>(o[i] / l, o[i + 1] / l);
   if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m * 0.69314718055994531f + logf(l);
 }
 

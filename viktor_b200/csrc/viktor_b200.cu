@@ -927,13 +927,11 @@ static SharedPlan shared_plan(int B, int H, int HK, int D, int P, int S, int max
     r.p.prefix_tiles = static_cast<int>(P + rows / 256);
     r.p.prefix_splits = wide_splits(std::max<int64_t>(P, (rows + 255) / 256) * HK, S, 148);
     r.p.prefix_chunk = ((S + r.p.prefix_splits - 1) / r.p.prefix_splits + 127) / 128 * 128;
-    r.p.prefix_slots = 2 * r.p.prefix_splits;
   } else {
     r.mt = rows > 16 * static_cast<int64_t>(P) ? 2 : 1;
     r.p.prefix_tiles = static_cast<int>(P + rows / (16 * r.mt));
     r.p.prefix_splits = splits_of(S, static_cast<int64_t>(r.p.prefix_tiles) * HK, 128, ctas);
     r.p.prefix_chunk = chunk_of(S, r.p.prefix_splits);
-    r.p.prefix_slots = r.p.prefix_splits;
   }
   r.p.tail_tiles = static_cast<int>((ratio + 15) / 16);
   const int64_t pieces = static_cast<int64_t>(B) * HK * r.p.tail_tiles;
@@ -963,7 +961,7 @@ static int shared_run(const sattn::Args& a, SharedPlan r, void* stream) {
     const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const uint64_t dims[4] = {D, static_cast<uint64_t>(a.HK), static_cast<uint64_t>(a.S), static_cast<uint64_t>(a.P)};
     const uint64_t strides[3] = {D * 2, static_cast<uint64_t>(a.stride_ks) * 2, static_cast<uint64_t>(a.stride_kb) * 2};
-    const uint32_t box[4] = {64, 1, 128, 1};
+    const uint32_t box[4] = {64, 1, sattn::Wide<D>::kPos, 1};
     if (!make_map(&mk, type, a.k_prefix, 4, dims, strides, box, true) || !make_map(&mv, type, a.v_prefix, 4, dims, strides, box, true))
       return VK_ERR_ARG;
     auto kern = sattn::wide_kernel<T, D>;
@@ -978,10 +976,11 @@ static int shared_run(const sattn::Args& a, SharedPlan r, void* stream) {
     rc = r.mt == 2 ? (r.wt == 1 ? shared_split<T, D, 2, 1>(a, r.p, n, stream) : shared_split<T, D, 2, 4>(a, r.p, n, stream))
                    : (r.wt == 1 ? shared_split<T, D, 1, 1>(a, r.p, n, stream) : shared_split<T, D, 1, 4>(a, r.p, n, stream));
   if (rc != VK_OK) return rc;
-  const int splits = r.p.prefix_slots + r.p.tail_splits;
+  const int splits = r.p.prefix_splits + r.p.tail_splits;
   const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H);
-  return splits > 16 ? launch(sattn::join_kernel<T, D, 8>, dim3(rows), dim3(256), 0, stream, 1, a, r.p, splits)
-                     : launch(sattn::join_kernel<T, D, 1>, dim3(rows), dim3(32), 0, stream, 1, a, r.p, splits);
+  // one warp per row and head, or eight where there are many splits and rows alone do not fill the SMs
+  return splits > 32 ? launch(sattn::join_kernel<T, D, 8>, dim3(rows), dim3(256), 0, stream, 1, a, r.p, splits)
+                     : launch(sattn::join_kernel<T, D, 1>, dim3(blocks_for(rows, 4)), dim3(128), 0, stream, 1, a, r.p, splits);
 }
 
 template <typename T, int VEC>
@@ -1017,7 +1016,7 @@ extern "C" {
 size_t vk_shared_attention_workspace_bytes(int B, int H, int HK, int D, int P, int S, int max_tail) {
   if (B <= 0 || H <= 0 || HK <= 0 || H % HK || D <= 0 || P <= 0 || S <= 0 || max_tail < 0) return 0;
   const SharedPlan r = shared_plan(B, H, HK, D, P, S, max_tail);
-  return static_cast<size_t>(r.p.prefix_slots + r.p.tail_splits) * B * H * (D + 2) * 4;
+  return static_cast<size_t>(r.p.prefix_splits + r.p.tail_splits) * B * H * (D + 2) * 4;
 }
 
 int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* k_prefix, const void* v_prefix,
@@ -1074,7 +1073,7 @@ int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* 
   r.p.tail_items = static_cast<int>(r.tail_items);
   r.p.scale_log2 = scale * 1.4426950408889634f;
   r.p.ws_o = static_cast<float*>(workspace);
-  r.p.ws_ml = reinterpret_cast<float2*>(r.p.ws_o + static_cast<size_t>(r.p.prefix_slots + r.p.tail_splits) * B * H * D);
+  r.p.ws_ml = reinterpret_cast<float2*>(r.p.ws_o + static_cast<size_t>(r.p.prefix_splits + r.p.tail_splits) * B * H * D);
   if (dtype == VK_BF16)
     return D == 64 ? shared_run<__nv_bfloat16, 64>(a, r, stream) : shared_run<__nv_bfloat16, 128>(a, r, stream);
   return D == 64 ? shared_run<__half, 64>(a, r, stream) : shared_run<__half, 128>(a, r, stream);

@@ -9,6 +9,8 @@ back to PyTorch.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ._lib import call, load
@@ -336,6 +338,11 @@ def _cache_strides(shape, stride):
     return sb, ss
 
 
+@functools.lru_cache(maxsize=256)
+def _shared_workspace(*sizes):
+    return load().vk_shared_attention_workspace_bytes(*sizes)
+
+
 def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k_pages, v_pages, page_table, tail_lens,
                             scale=None, out=None, return_lse=False, workspace=None):
     """Attention of one query token per row over a prefix that a group of rows shares and the row's own tail.
@@ -381,10 +388,11 @@ def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k
     _need(one == 1 and (H == 1 or sh == D), "the heads of a row of q must be contiguous")
     _need(stride_q >= H * D and stride_q % 8 == 0, "the rows of q must be 16-byte aligned and must not overlap")
     kb, ks = _cache_strides(prefix_shape, k_prefix.stride())
-    _need((kb, ks) == _cache_strides(prefix_shape, v_prefix.stride()), "k_prefix and v_prefix must have the same strides")
     pp, ps = _cache_strides(pages_shape, k_pages.stride())
-    _need((pp, ps) == _cache_strides(pages_shape, v_pages.stride()) and ps == HK * D, "pages must be contiguous, with the same "
-          "strides in k and v")
+    _need(v_prefix.stride() == k_prefix.stride() or (kb, ks) == _cache_strides(prefix_shape, v_prefix.stride()),
+          "k_prefix and v_prefix must have the same strides")
+    _need(ps == HK * D and (v_pages.stride() == k_pages.stride() or (pp, ps) == _cache_strides(pages_shape, v_pages.stride())),
+          "pages must be contiguous, with the same strides in k and v")
     scale = D ** -0.5 if scale is None else float(scale)
     _need(0.0 < scale < float("inf"), "scale must be positive and finite")
     q_at = q.data_ptr()
@@ -397,7 +405,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k
         _need(B == 0 or out_at + 2 * B * H * D <= q_at or out_at >= q_at + 2 * ((B - 1) * stride_q + H * D), "out must not overlap q")
     lse = torch.empty(B, H, dtype=torch.float32, device=device) if return_lse else None
     if B:
-        nbytes = load().vk_shared_attention_workspace_bytes(B, H, HK, D, P, S, max_pages * page)
+        nbytes = _shared_workspace(B, H, HK, D, P, S, max_pages * page)
         if workspace is None:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         elif not workspace.is_contiguous() or workspace.nbytes < nbytes:
