@@ -6,6 +6,10 @@
 // A row with nothing to attend gives 0 (lse -inf); rows behind the last group are not touched.
 #pragma once
 
+#ifndef VK_POLY
+#define VK_POLY 0x22
+#endif
+
 #include <type_traits>
 
 #include "vk_common.cuh"
@@ -29,15 +33,6 @@ struct Args {
   int B, H, HK, P, S, n_pages, page_shift, max_pages;
 };
 
-// Reports group offsets that do not ascend from 0 to at most B.  Spread over the threads of the grid.
-VK_DEV void check_offsets(const Args& a) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t g = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; g < a.P; g += step) {
-    const int lo = a.offsets[g], hi = a.offsets[g + 1];
-    if (lo > hi || hi > a.B || (g == 0 && lo != 0)) raise_error(ERR_BOUNDS);
-  }
-}
-
 constexpr int kThreads = 128;  // 4 warps
 constexpr int kStages = 3;     // of each warp's own ring
 
@@ -49,6 +44,7 @@ struct Plan {
   int tail_tiles;     // tiles of 16 heads of one (row, KV head)
   int tail_splits, tail_chunk;
   int prefix_items, tail_items;
+  bool behind_wide;   // launched right behind wide_kernel of the same call
   float scale_log2;
   float* ws_o;        // [prefix_splits + tail_splits][B * H][D]
   float2* ws_ml;      // [prefix_splits + tail_splits][B * H]: maximum (of scores in base 2) and sum
@@ -390,60 +386,42 @@ VK_DEV void run_item(const Args& a, const Plan& pl, uint8_t* smem, const Source<
   store_partial<D, MT, WI>(a, pl, smem, split, b0, kvh, r, x0, x1, o, m, l);
 }
 
-// The rows of a prefix item: rows x0 .. x1 - 1 (numbered as in load_q) of the group g; x0 >= x1: none.
+// The rows of a prefix item: rows x0 .. x1 - 1 (numbered as in load_q) of the group g, whose prefix has len positions; x0 >= x1:
+// none.
 struct Rows {
-  int g, b0, kvh, split, x0, x1;
+  int g, b0, len, kvh, split, x0, x1;
 };
-// The item of this CTA of `threads` threads with tiles of kRows rows.  found: one shared word.
+// The item of this CTA of `threads` threads with tiles of kRows rows; found: shared.  Every thread looks at its groups; the one
+// whose group's tiles hold this one (group g's begin at floor(offset_g * r / kRows) + g) says so: one round of loads.
 template <int kRows, int threads>
-VK_DEV Rows find_rows(const Args& a, const Plan& pl, int* found) {
+VK_DEV Rows find_rows(const Args& a, const Plan& pl, Rows* found) {
   const int r = a.H / a.HK;
-  Rows w{};
   int item = blockIdx.x;
-  w.split = item % pl.prefix_splits;
+  const int split = item % pl.prefix_splits;
   item /= pl.prefix_splits;
-  w.kvh = item % a.HK;
-  const int tile = item / a.HK;
-  // the group whose tiles hold this one: the last that begins at or before it
-  if (threadIdx.x == 0) *found = 0;
+  const int kvh = item % a.HK, tile = item / a.HK;
+  if (threadIdx.x == 0) found->x0 = found->x1 = 0;
   __syncthreads();
-  int n = 0;
-  for (int g = threadIdx.x; g < a.P; g += threads) n += static_cast<int64_t>(a.offsets[g]) * r / kRows + g <= tile;
-  for (int x = 16; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
-  if ((threadIdx.x & 31) == 0) atomicAdd(found, n);
+  for (int g = threadIdx.x; g < a.P; g += threads) {
+    const int lo = a.offsets[g], hi = a.offsets[g + 1], length = a.prefix_lens[g];
+    if (lo < 0 || lo > hi || hi > a.B || (g == 0 && lo != 0)) {
+      raise_error(ERR_BOUNDS);  // they have to ascend from 0 to at most B
+      continue;
+    }
+    const int first = static_cast<int>(static_cast<int64_t>(lo) * r / kRows) + g;
+    const int64_t x0 = static_cast<int64_t>(tile - first) * kRows, all = static_cast<int64_t>(hi - lo) * r;
+    if (x0 < 0 || x0 >= all) continue;
+    const int len = checked_len(length, a.S);
+    *found = Rows{g, lo, len, kvh, split, static_cast<int>(x0), static_cast<int>(x0 + kRows < all ? x0 + kRows : all)};
+  }
   __syncthreads();
-  w.g = *found - 1;
-  if (w.g < 0) return w;
-  w.b0 = a.offsets[w.g];
-  const int b1 = min(a.offsets[w.g + 1], a.B);
-  if (w.b0 < 0 || w.b0 >= b1) return w;
-  const int64_t x0 = (tile - static_cast<int64_t>(w.b0) * r / kRows - w.g) * kRows, all = static_cast<int64_t>(b1 - w.b0) * r;
-  if (x0 < 0 || x0 >= all) return w;
-  w.x0 = static_cast<int>(x0);
-  w.x1 = static_cast<int>(x0 + kRows < all ? x0 + kRows : all);
-  return w;
+  return *found;
 }
 
-// MT: 16-row tiles of a prefix item.  WT: warps of a tail item.
-template <typename T, int D, int MT, int WT>
-__global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int found;
-  const int r = a.H / a.HK;
-  pdl_wait();
-  check_offsets(a);
-  if (static_cast<int>(blockIdx.x) < pl.prefix_items) {
-    const Rows w = find_rows<16 * MT, kThreads>(a, pl, &found);
-    if (w.x0 >= w.x1) return;
-    Source<T> s{};
-    s.k = static_cast<const T*>(a.k_prefix) + w.g * a.stride_kb + w.kvh * D;
-    s.v = static_cast<const T*>(a.v_prefix) + w.g * a.stride_kb + w.kvh * D;
-    s.stride = a.stride_ks;
-    const int len = checked_len(a.prefix_lens[w.g], a.S), begin = w.split * pl.prefix_chunk;
-    run_item<T, D, MT, 4, false>(a, pl, smem, s, w.split, begin, min(begin + pl.prefix_chunk, len), w.b0, w.kvh, r, w.x0, w.x1);
-    return;
-  }
-  const int per = WT == 1 ? 4 : 1;  // items of a CTA
+// The tail item of this CTA, or of this warp.
+template <typename T, int D, int WT>
+VK_DEV void tail_item(const Args& a, const Plan& pl, uint8_t* smem) {
+  const int r = a.H / a.HK, per = WT == 1 ? 4 : 1;  // items of a CTA
   int item = (blockIdx.x - pl.prefix_items) * per + (WT == 1 ? threadIdx.x >> 5 : 0);
   if (item >= pl.tail_items) return;
   const int split = item % pl.tail_splits;
@@ -465,19 +443,47 @@ __global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
                               tile * 16, min(tile * 16 + 16, r));
 }
 
+// MT: 16-row tiles of a prefix item.  WT: warps of a tail item.
+template <typename T, int D, int MT, int WT>
+__global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Rows found;
+  // Tails do not read what wide_kernel writes, and wide_kernel lets this one start only after its own wait for what came
+  // before: so behind it the tails run at once, and the wait comes last, for the kernel that joins both.
+  if (!pl.behind_wide) pdl_wait();
+  pdl_launch_dependents();
+  if (static_cast<int>(blockIdx.x) < pl.prefix_items) {
+    const Rows w = find_rows<16 * MT, kThreads>(a, pl, &found);
+    if (w.x0 < w.x1) {
+      Source<T> s{};
+      s.k = static_cast<const T*>(a.k_prefix) + w.g * a.stride_kb + w.kvh * D;
+      s.v = static_cast<const T*>(a.v_prefix) + w.g * a.stride_kb + w.kvh * D;
+      s.stride = a.stride_ks;
+      const int begin = w.split * pl.prefix_chunk;
+      run_item<T, D, MT, 4, false>(a, pl, smem, s, w.split, begin, min(begin + pl.prefix_chunk, w.len), w.b0, w.kvh, a.H / a.HK,
+                                   w.x0, w.x1);
+    }
+  } else {
+    tail_item<T, D, WT>(a, pl, smem);
+  }
+  if (pl.behind_wide) pdl_wait();
+}
+
 // ---- wide groups -------------------------------------------------------------------------------------------------
 // Prefix attention of up to 256 rows of one group and KV head on the 5th-generation tensor cores, one CTA per SM:
 //   warp 0      TMA: 64-position tiles of K and V, one after another, into a ring of units
-//   warp 1      MMA issue (one lane); two streams s = 0, 1, each with two 128 x 64 score buffers and a 128 x D result in TMEM:
-//                 S_s = Q K_j^T, then, once the softmax has put P over S_s, O_s += P V_j
+//   warps 1, 10 MMA issue of two streams s = 0, 1, each with 128 x 64 scores, two buffers of probabilities and a 128 x D result in
+//               TMEM: S_s = Q K_j^T, then, once the softmax has put P there, O_s += P V_j
 //   warps 2-5   softmax of stream 0, one row per thread; warps 6-9 of stream 1
 // More than 128 rows: the streams are the two halves of the rows and share every tile.  Otherwise they take the even and the
-// odd tiles for the same rows and are joined at the end.  A stream's next scores are ready while its softmax works: with one
-// buffer of 128 positions the softmax waited for the tensor cores half of the time (181 us against ... for 256 rows x 32 heads
-// on 32768 positions).
+// odd tiles for the same rows and are joined at the end.
+//
+// A batch of MMAs takes some 600 cycles more from issue to completion than its work (256 cycles), so nothing a stream's softmax
+// waits for may hang on its last result: the scores of tile c + 1 are issued as soon as those of c are in registers, and P
+// has a place of its own, twice.  @@WIDE@@
 template <int D>
 struct Wide {
-  static constexpr int kThreads = 320;
+  static constexpr int kThreads = 352;
   static constexpr int kRows = 128;                     // of a stream
   static constexpr int kPos = 64;
   static constexpr int kUnit = kPos * D * 2;            // bytes of a K or V tile
@@ -487,7 +493,7 @@ struct Wide {
   static constexpr int kRing = 2 * kQ;                  // behind the queries
   static constexpr int kBars = kRing + kUnits * kUnit;
   static constexpr int kSmem = kBars + 512 + 1024;
-  static constexpr uint32_t kColO = 256;                // S_s: 128 s + 64 (tile & 1); O_s: kColO + D s
+  static constexpr uint32_t kColO = 256;                // S_s: 128 s; P_s: 128 s + 64 + 32 (tile & 1); O_s: kColO + D s
   static constexpr uint32_t kCols = 512;
 };
 
@@ -510,6 +516,33 @@ VK_DEV uint32_t pack2<__half>(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Largest of three, NaN if one is.
+VK_DEV float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two values, -inf..9, on the FMA pipes, for a part of the probabilities: the SM takes 16 exponentials a cycle but 128 FMAs.
+// x is split into a whole number n (by adding 1.5 * 2^23) and f in -0.5..0.5; 2^f by the polynomial of degree 5 with the
+// smallest largest relative error on that range (fitted in float64 by reweighted least squares: 2^-23.7; in float32
+// arithmetic 2^-22.1); n goes into the exponent bits.  Below -127 the result is 2^-149.  NaN gives some number: the caller
+// looks for it in the maximum.
+VK_DEV float2 poly_exp2(float2 x) {
+  x = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
+  const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
+  const float2 t = __fadd2_rn(x, magic), n = __fadd2_rn(t, minus);
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 p = make_float2(0.0013276472454890609f, 0.0013276472454890609f);
+  p = __ffma2_rn(p, f, make_float2(0.009675540961325169f, 0.009675540961325169f));
+  p = __ffma2_rn(p, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
+  p = __ffma2_rn(p, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+  p = __ffma2_rn(p, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+  p = __ffma2_rn(p, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Args a, Plan pl) {
@@ -520,22 +553,22 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + W::kBars);
   uint64_t* u_full = q_full + 1;
   uint64_t* u_empty = u_full + W::kUnits;
-  uint64_t* s_full = u_empty + W::kUnits;  // [2][2] stream, buffer: scores in TMEM
-  uint64_t* p_full = s_full + 4;           // [2][2] probabilities in TMEM, result rescaled
-  uint64_t* o_full = p_full + 4;           // [2][2] stream, tile & 1: product done
+  uint64_t* s_full = u_empty + W::kUnits;  // [2] scores in TMEM
+  uint64_t* s_free = s_full + 2;           // [2] scores read
+  uint64_t* p_full = s_free + 2;           // [2][2] stream, tile & 1: probabilities in TMEM, result rescaled
+  uint64_t* o_full = p_full + 4;           // [2][2] product done
   uint64_t* tmem_free = o_full + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_free + 1);
-  int* found = reinterpret_cast<int*>(tmem_slot + 1);
+  Rows* found = reinterpret_cast<Rows*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int r = a.H / a.HK;
 
   pdl_wait();
-  check_offsets(a);
+  pdl_launch_dependents();
   const Rows w = find_rows<2 * W::kRows, W::kThreads>(a, pl, found);
   if (w.x0 >= w.x1) return;
   const bool both = w.x1 - w.x0 > W::kRows;  // the streams share the tiles
-  const int len = checked_len(a.prefix_lens[w.g], a.S), begin = w.split * pl.prefix_chunk;
-  const int end = min(begin + pl.prefix_chunk, len);
+  const int begin = w.split * pl.prefix_chunk, end = min(begin + pl.prefix_chunk, w.len);
   if (begin >= end) {
     store_nothing(a, pl, w.split, w.b0, w.kvh, r, w.x0, w.x1, threadIdx.x, W::kThreads);
     return;
@@ -546,11 +579,14 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     mbar_init(q_full, 8);
     for (int i = 0; i < W::kUnits; ++i) {
       mbar_init(&u_full[i], 1);
-      mbar_init(&u_empty[i], 1);
+      mbar_init(&u_empty[i], both ? 2 : 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);  // (one for each buffer: the softmax may be a tile ahead of the products)
+      mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(tmem_free, 8);
@@ -584,8 +620,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
           tma_load_4d(to + c * W::kSub, map, &u_full[slot], c * 64, w.kvh, begin + (u >> 1) * W::kPos, w.g);
       }
     }
-  } else if (warp == 1) {
-    // ---------------- MMA issue: the whole warp in step, one lane issues ----------------
+  } else if (warp == 1 || warp == 10) {
+    // ---------------- MMA issue of one stream: the whole warp in step, one lane issues ----------------
+    const int s = warp == 1 ? 0 : 1;
     constexpr uint32_t kTypes = kF16 ? (1u << 7) | (1u << 10) : 0u;  // fp16 operands: clear the bf16 format bits
     constexpr uint32_t idesc_s = idesc_bf16_f32(W::kRows, W::kPos) & ~kTypes;
     constexpr uint32_t idesc_o = (idesc_bf16_f32(W::kRows, D) & ~kTypes) | (1u << 16);  // V is MN-major
@@ -612,31 +649,35 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       }
     };
     Cursor k{0, 0}, v{1, 0};
-    const auto scores = [&](int s, int c) {  // the c-th tile of stream s; its K is there
-      const uint64_t qd = sdesc_tile(base + (share ? s : 0) * W::kQ, 16);
+    const int mine = share ? n : (n + 1 - s) / 2, step = share ? 1 : 2;  // tiles of this stream
+    if (!share && s == 1) {
+      k.next();
+      v.next();
+    }
+    const uint64_t qd = sdesc_tile(base + (share ? s : 0) * W::kQ, 16);
+    const auto release = [&](Cursor& u) {
+      umma_commit_if(one, at(u_empty, u.slot));
+      for (int i = 0; i < step; ++i) u.next();
+    };
+    const auto scores = [&] {  // of the stream's next tile
+      wait(&u_full[k.slot], k.phase);
+      tc_fence_after();
       const uint64_t kd = sdesc_tile(base + W::kRing + k.slot * W::kUnit, 16);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
-        umma_ss_if(one, tm + s * 128 + (c & 1) * 64, qd + ks / 4 * (16384 / 16) + 2 * (ks % 4), kd + ks / 4 * (W::kSub / 16) + 2 * (ks % 4),
+        umma_ss_if(one, tm + s * 128, qd + ks / 4 * (16384 / 16) + 2 * (ks % 4), kd + ks / 4 * (W::kSub / 16) + 2 * (ks % 4),
                    idesc_s, ks != 0);
-      umma_commit_if(one, at(s_full, 2 * s + (c & 1)));
+      umma_commit_if(one, at(s_full, s));
+      release(k);
     };
-    const auto product = [&](int s, int c) {  // its V is there
-      wait(&p_full[2 * s + (c & 1)], (c >> 1) & 1);
-      tc_fence_after();
-      const uint64_t vd = sdesc_tile(base + W::kRing + v.slot * W::kUnit, W::kSub);
-#pragma unroll
-      for (int ks = 0; ks < W::kPos / 16; ++ks)
-        umma_ts_if(one, tm + W::kColO + s * D, tm + s * 128 + (c & 1) * 64 + ks * 8, vd + ks * (2048 / 16), idesc_o, (c | ks) != 0);
-      umma_commit_if(one, at(o_full, 2 * s + (c & 1)));
-    };
-    const auto wait_k = [&] {
-      wait(&u_full[k.slot], k.phase);
-      tc_fence_after();
-    };
-    const auto wait_v = [&](int j) {
+    if (mine > 0) scores();
+    for (int c = 0; c < mine; ++c) {
+      if (c + 1 < mine) {
+        wait(&s_free[s], c & 1);
+        scores();
+      }
       wait(&u_full[v.slot], v.phase);
-      if (j == n - 1 && last < W::kPos) {  // what lies behind the prefix may hold anything, and 0 * NaN is NaN
+      if (last < W::kPos && c * step + (share ? 0 : s) == n - 1) {  // what lies behind the prefix may hold anything, and 0 * NaN is NaN
         for (int i = lane; i < (W::kPos - last) * (D / 8); i += 32) {
           const int pos = last + i / (D / 8), ch = i % (D / 8);
           *reinterpret_cast<uint4*>(smem + W::kRing + v.slot * W::kUnit + ch / 8 * W::kSub + pos * 128 + ch % 8 * 16) =
@@ -645,52 +686,15 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         fence_proxy_async();
         __syncwarp();
       }
-    };
-    const auto release = [&](Cursor& u) {
-      umma_commit_if(one, at(u_empty, u.slot));
-      u.next();
-    };
-    // scores run two tiles of a stream ahead of its products: into the buffer that the product before them has left
-    if (share) {
-      for (int j = 0; j < 2 && j < n; ++j) {
-        wait_k();
-        scores(0, j);
-        scores(1, j);
-        release(k);
-      }
-      for (int j = 0; j < n; ++j) {
-        const bool more = j + 2 < n;
-        wait_v(j);
-        product(0, j);
-        if (more) {
-          wait_k();
-          scores(0, j + 2);
-        }
-        product(1, j);
-        release(v);
-        if (more) {
-          scores(1, j + 2);
-          release(k);
-        }
-        if (__any_sync(0xffffffffu, late)) break;
-      }
-    } else {
-      for (int j = 0; j < 4 && j < n; ++j) {
-        wait_k();
-        scores(j & 1, j >> 1);
-        release(k);
-      }
-      for (int j = 0; j < n; ++j) {
-        wait_v(j);
-        product(j & 1, j >> 1);
-        release(v);
-        if (j + 4 < n) {
-          wait_k();
-          scores(j & 1, (j >> 1) + 2);
-          release(k);
-        }
-        if (__any_sync(0xffffffffu, late)) break;
-      }
+      wait(&p_full[2 * s + (c & 1)], (c >> 1) & 1);
+      tc_fence_after();
+      const uint64_t vd = sdesc_tile(base + W::kRing + v.slot * W::kUnit, W::kSub);
+#pragma unroll
+      for (int ks = 0; ks < W::kPos / 16; ++ks)
+        umma_ts_if(one, tm + W::kColO + s * D, tm + s * 128 + 64 + (c & 1) * 32 + ks * 8, vd + ks * (2048 / 16), idesc_o, (c | ks) != 0);
+      umma_commit_if(one, at(o_full, 2 * s + (c & 1)));
+      release(v);
+      if (__any_sync(0xffffffffu, late)) break;
     }
     if (late) raise_error(ERR_WAIT_FULL);
   } else {
@@ -698,15 +702,25 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     const int s = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int x = w.x0 + (both ? s * W::kRows : 0) + row;  // this thread's row of the group
     const bool used = x < w.x1;
-    const int h = w.kvh * r + x % r;
-    // Q: this thread's row of stream s's queries (queries of both: the streams load a half of the columns each)
+    const int token = w.b0 + x / r, h = w.kvh * r + x % r;
+    // the stream's queries (of joined streams each loads a half of the rows): a warp takes its rows one after another, so that its
+    // lanes read whole rows (a row per thread: 5 us)
     {
-      const T* qp = static_cast<const T*>(a.q) + (used ? (w.b0 + x / r) * a.stride_q + h * D : 0);
-      uint8_t* to = smem + (both ? s : 0) * W::kQ + row * 128;
-      const int c0 = both ? 0 : s * (D / 16), c1 = both ? D / 8 : c0 + D / 16;
-      for (int c = c0; c < c1; ++c) {
-        const uint4 v = used ? *reinterpret_cast<const uint4*>(qp + c * 8) : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(to + c / 8 * 16384 + (((c & 7) ^ (row & 7)) << 4)) = v;
+      constexpr int kChunks = D / 8, kAt = 32 / kChunks;  // 16-byte chunks of a row, rows at a time
+      const int64_t mine = used ? token * a.stride_q + h * D : -1;
+      uint4 v[kChunks];
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int64_t off = __shfl_sync(0xffffffffu, mine, i * kAt + lane / kChunks);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (off >= 0 && (both || i * 2 / kChunks == s))
+          v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + off) + lane % kChunks);
+      }
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int ro = quarter * 32 + i * kAt + lane / kChunks, c = lane % kChunks;
+        if (both || i * 2 / kChunks == s)
+          *reinterpret_cast<uint4*>(smem + (both ? s : 0) * W::kQ + c / 8 * 16384 + ro * 128 + (((c & 7) ^ (ro & 7)) << 4)) = v[i];
       }
       fence_proxy_async();
       __syncwarp();
@@ -717,30 +731,35 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     const int mine = both ? tiles : (tiles + 1 - s) / 2;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    // The product of the c-th tile is done.  Called when the scores of tile c or c + 1 are there, which were issued behind the
-    // product c - 2: of its barrier's phases only the one waited for can be open.
+    const uint32_t ts = tmem + s * 128 + lanes;
+    // The product of the c-th tile is done.  The scores of tile c are issued behind the product c - 2: when they are there, its
+    // buffer of P is free, and of the phases of o_full[c & 1] none but that of tile c - 1 or c can be open.
     auto wait_product = [&](int c) { return __all_sync(0xffffffffu, mbar_wait(&o_full[2 * s + (c & 1)], (c >> 1) & 1)); };
     for (int c = 0; c < mine; ++c) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * s + (c & 1)], (c >> 1) & 1));
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], c & 1));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t ts = tmem + s * 128 + (c & 1) * 64 + lanes;
       float v[W::kPos];
 #pragma unroll
       for (int i = 0; i < W::kPos; i += 16) tmem_ld16(ts + i, v + i);
       tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_free[s]);
       const int left = end - begin - (both ? c : 2 * c + s) * W::kPos;
       if (left < W::kPos) {
 #pragma unroll
         for (int i = 0; i < W::kPos; ++i)
           if (i >= left) v[i] = -INFINITY;
       }
-      float mx4[4] = {v[0], v[1], v[2], v[3]};
+      float mx4[4];
 #pragma unroll
-      for (int i = 4; i < W::kPos; i += 8)
+      for (int k = 0; k < 4; ++k) {
+        mx4[k] = max3_nan(v[k], v[k + 4], v[k + 8]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx4[k] = i + 4 < W::kPos ? fmaxf(fmaxf(mx4[k], v[i + k]), v[(i + 4 + k) % W::kPos]) : fmaxf(mx4[k], v[i + k]);
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * pl.scale_log2;
+        for (int i = 12; i < W::kPos; i += 8) mx4[k] = i + 4 < W::kPos ? max3_nan(mx4[k], v[i + k], v[i + k + 4]) : max3_nan(mx4[k], v[i + k], v[i + k]);
+      }
+      const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * pl.scale_log2;
       // the reference maximum follows only when it is passed by more than 2^8: probabilities up to 256 round as well
       const float m_new = mx > m + 8.f || m == -INFINITY ? fmaxf(m, mx) : m;
       const float mu = m_new == -INFINITY ? 0.f : m_new;
@@ -752,11 +771,11 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float2 t = __ffma2_rn(make_float2(v[c0 + i], v[c0 + i + 1]), sc2, nm2);
-          const float2 p = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+          const float2 p = (VK_POLY >> (i >> 1 & 7)) & 1 ? poly_exp2(t) : make_float2(fast_exp2(t.x), fast_exp2(t.y));
           rs4[(i >> 1) & 3] = __fadd2_rn(rs4[(i >> 1) & 3], p);
           pk[i / 2] = pack2<T>(p.x, p.y);
         }
-        tmem_st16(ts + c0 / 2, pk);
+        tmem_st16(ts + 64 + (c & 1) * 32 + c0 / 2, pk);
       }
       const float2 rs2 = __fadd2_rn(__fadd2_rn(rs4[0], rs4[1]), __fadd2_rn(rs4[2], rs4[3]));
       const float alpha = fast_exp2(m - mu);
@@ -782,6 +801,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[2 * s + (c & 1)]);
       l = alpha * l + rs2.x + rs2.y;
+      if (!(mx < INFINITY)) l = NAN;  // a score that is NaN or inf
       m = m_new;
     }
     if (mine > 0 && ok) ok = wait_product(mine - 1);
@@ -808,7 +828,6 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       asm volatile("bar.sync 1, 256;" ::: "memory");
     }
     if (both || s == 0) {
-      const int64_t slot = (static_cast<int64_t>(w.split) * a.B + w.b0 + x / r) * a.H + h;
       float f0 = 1.f, f1 = 0.f;
       if (!both && tiles > 1) {
         const float2 ml = other_ml[row];
@@ -818,21 +837,37 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         l = l * f0 + ml.y * f1;
         m = mn;
       }
+      // the warp's 32 rows, a half of the columns at a time, turned in shared memory so that a row is written in one piece
+      // (straight from the threads' rows: 5 us more for every CTA).  Its place: this warp's part of the stream's queries, or of
+      // the ring behind other_ml where the queries' place holds the other stream's result.
+      float4* turn = reinterpret_cast<float4*>(smem + (both ? s * W::kQ : W::kRing + W::kUnit) + quarter * (W::kQ / 4));
+      constexpr int kC = D / 8;  // float4s of half a row
+      const int64_t slot = (static_cast<int64_t>(w.split) * a.B + token) * a.H + h;
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        float o[32];
-        tmem_ld16(to + c0, o);
-        tmem_ld16(to + c0 + 16, o + 16);
-        tmem_wait_ld();
-        if (!both && tiles > 1) {
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + other[(c0 + i) * 128 + row] * f1;
-        }
-        if (used) {
+        for (int c0 = 0; c0 < D / 2; c0 += 32) {
+          float o[32];
+          tmem_ld16(to + half * (D / 2) + c0, o);
+          tmem_ld16(to + half * (D / 2) + c0 + 16, o + 16);
+          tmem_wait_ld();
+          if (!both && tiles > 1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + other[(half * (D / 2) + c0 + i) * 128 + row] * f1;
+          }
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(pl.ws_o + slot * D + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            turn[lane * kC + (((c0 + i) / 4) ^ (lane & 7))] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
+        __syncwarp();
+#pragma unroll 4
+        for (int i = lane; i < 32 * kC; i += 32) {
+          const int ro = i / kC, c = i % kC;
+          const int64_t to_slot = __shfl_sync(0xffffffffu, used ? slot : -1, ro);
+          if (to_slot >= 0)
+            *reinterpret_cast<float4*>(pl.ws_o + to_slot * D + half * (D / 2) + c * 4) = turn[ro * kC + (c ^ (ro & 7))];
+        }
+        __syncwarp();
       }
       if (used) pl.ws_ml[slot] = make_float2(m, l);
     }

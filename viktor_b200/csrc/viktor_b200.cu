@@ -969,6 +969,7 @@ static int shared_run(const sattn::Args& a, SharedPlan r, void* stream) {
     rc = launch(kern, dim3(static_cast<unsigned>(r.prefix_items)), dim3(sattn::Wide<D>::kThreads), sattn::Wide<D>::kSmem, stream, 1,
                 mk, mv, a, r.p);
     r.prefix_items = 0;
+    r.p.behind_wide = true;
   }
   r.p.prefix_items = static_cast<int>(r.prefix_items);
   const unsigned n = static_cast<unsigned>(r.prefix_items + tails);
