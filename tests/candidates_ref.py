@@ -37,8 +37,9 @@ def attend_bounds(out, spread, span, n, D, dtype):
 
     Scores: products of two 16-bit values are exact in float32; D of them are summed, so a score is off by at most
     (D + 2) 2^-23 span, and times log2(e), minus the maximum (|z| <= span): another 4 2^-24 span.  exp2 is off by 2^-21
-    relative.  So every p is off by delta = (D + 4) 2^-23 span + 2^-21 relative, before it is rounded to the type (u),
-    with the sum of the same values below it: 2 (delta + u) at most for p_j / sum p.  The n products are summed in chains
+    relative.  So every p is off by delta = (D + 4) 2^-23 span + 2^-21 relative, and the sum of them by no more.  Only the product
+    with V takes p rounded
+    to the type (u): 2 (delta + u) at most for p_j / sum p; the log of the sum is off by delta, and 2^-20 for the joins and the log.  The n products are summed in chains
     of at most n / 16 + 64 float32 additions (a matrix instruction takes 16 positions at least one at a time: n / 16 + 16
     steps, then the joins), (n / 16 + 64) 2^-23 of spread, twice (values and sum).  The result is rounded once: u |out|."""
     u = torch.finfo(dtype).eps / 2
@@ -46,7 +47,7 @@ def attend_bounds(out, spread, span, n, D, dtype):
     chain = 2 * (n / 16 + 64) * 2.0 ** -23
     # a value below the type's smallest normal is off by up to half its smallest step
     small = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
-    return (2 * (delta[..., None] + u) + chain) * spread * 1.01 + u * out.abs() + small, delta + u + chain + 2.0 ** -20
+    return (2 * (delta[..., None] + u) + chain) * spread * 1.01 + u * out.abs() + small, delta + chain + 2.0 ** -20
 
 
 class PoolRef:

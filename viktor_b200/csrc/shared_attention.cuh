@@ -6,10 +6,6 @@
 // A row with nothing to attend gives 0 (lse -inf); rows behind the last group are not touched.
 #pragma once
 
-#ifndef VK_POLY
-#define VK_POLY 0x22
-#endif
-
 #include <type_traits>
 
 #include "vk_common.cuh"
@@ -34,7 +30,7 @@ struct Args {
 };
 
 constexpr int kThreads = 128;  // 4 warps
-constexpr int kStages = 3;     // of each warp's own ring
+constexpr int kStages = 2;     // of each warp's own ring
 
 // Work of one launch: prefix items (tile of rows, KV head, chunk) first, then tail items (row, KV head, tile of heads, chunk).
 // Partial results go to slot [split][b * H + h], prefix chunks first.
@@ -65,24 +61,23 @@ VK_DEV void mma_16816<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two probabilities rounded to the type, and in *sum the sum of what they became.
+// Two values rounded to the type.
 template <typename T>
-VK_DEV uint32_t pack_p(float x, float y, float* sum);
+VK_DEV uint32_t pack2(float x, float y);
 template <>
-VK_DEV uint32_t pack_p<__nv_bfloat16>(float x, float y, float* sum) {
-  const uint32_t u = pack_bf16x2(x, y);
-  *sum += bf16_lo(u) + bf16_hi(u);
-  return u;
+VK_DEV uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  return pack_bf16x2(x, y);
 }
 template <>
-VK_DEV uint32_t pack_p<__half>(float x, float y, float* sum) {
+VK_DEV uint32_t pack2<__half>(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  *sum += f.x + f.y;
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 16 bytes from global to shared memory, zeros where !use.
+// 16 bytes from global to shared memory; the second form: zeros where !use.
+VK_DEV void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 VK_DEV void cp_async16(uint32_t dst, const void* src, bool use) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(use ? 16 : 0) : "memory");
 }
@@ -116,25 +111,44 @@ struct Source {
 };
 
 // Loads positions p .. p + kPos - 1 (those at or past end: zeros) into one stage.  page: this lane's page id, that of
-// position p + lane.
+// position p + lane.  Where a tile lies in one piece (a prefix, or pages of at least kPos tokens) a lane's addresses are one base
+// and constant steps.
 template <typename T, int D, bool PAGED>
 VK_DEV void load_tile(const Source<T>& s, uint32_t stage, int p, int end, int page) {
-  constexpr int kChunks = D / 8, kRows = 32 / kChunks, kLoads = Tile<D>::kPos / kRows;
-  const int lane = threadIdx.x & 31, c = lane % kChunks, r0 = lane / kChunks;
+  constexpr int kChunks = D / 8, kRows = 32 / kChunks, kPos = Tile<D>::kPos, kLoads = kPos / kRows;
+  const int lane = threadIdx.x & 31, c = lane % kChunks, r0 = lane / kChunks, mask = (1 << s.page_shift) - 1;
+  if (!PAGED || mask >= kPos - 1) {
+    int64_t off = PAGED ? __shfl_sync(0xffffffffu, page, 0) * s.stride_page + static_cast<int64_t>(p & mask) * s.stride : p * s.stride;
+    off += r0 * s.stride + c * 8;
+    const T *k = s.k + off, *v = s.v + off;
+    const int64_t step = kRows * s.stride;
+    if (p + kPos <= end) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int r = r0 + i * kRows, pos = p + r;
-    int64_t off;
-    if (PAGED) {
-      const int pg = __shfl_sync(0xffffffffu, page, r);
-      off = pg * s.stride_page + static_cast<int64_t>(pos & ((1 << s.page_shift) - 1)) * s.stride;
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t to = stage + Tile<D>::at(r0 + i * kRows, c);
+        cp_async16(to, k + i * step);
+        cp_async16(to + Tile<D>::kHalf, v + i * step);
+      }
     } else {
-      off = pos * s.stride;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t to = stage + Tile<D>::at(r0 + i * kRows, c);
+        const bool use = p + r0 + i * kRows < end;
+        cp_async16(to, use ? k + i * step : s.k, use);
+        cp_async16(to + Tile<D>::kHalf, use ? v + i * step : s.v, use);
+      }
     }
-    const bool use = pos < end;
-    off = use ? off + c * 8 : 0;
-    cp_async16(stage + Tile<D>::at(r, c), s.k + off, use);
-    cp_async16(stage + Tile<D>::kHalf + Tile<D>::at(r, c), s.v + off, use);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = r0 + i * kRows, pos = p + r;
+      const int pg = __shfl_sync(0xffffffffu, page, r);
+      const bool use = pos < end;
+      const int64_t off = use ? pg * s.stride_page + static_cast<int64_t>(pos & mask) * s.stride + c * 8 : 0;
+      const uint32_t to = stage + Tile<D>::at(r, c);
+      cp_async16(to, s.k + off, use);
+      cp_async16(to + Tile<D>::kHalf, s.v + off, use);
+    }
   }
 }
 
@@ -211,19 +225,19 @@ VK_DEV void attend(const Source<T>& s, uint32_t ring, int begin, int end, int fi
           mma_16816<T>(sc[a][n + 1], q[a][ks], b[2], b[3]);
         }
       }
-    // ---- softmax in base 2; the sum is that of the rounded probabilities, which the product below uses ----
-    const int p0 = begin + t * kPos;
-    const bool partial = p0 + kPos > end;
+    // ---- softmax in base 2; probabilities are rounded to the type for the product below, their sum is not ----
+    const int pos0 = begin + t * kPos;
+    const bool partial = pos0 + kPos > end;
     uint32_t pr[MT][kN][2];
 #pragma unroll
     for (int a = 0; a < MT; ++a) {
       float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
+        if (partial) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[a][n][e] *= scale_log2;
-          if (partial && p0 + n * 8 + 2 * t4 + (e & 1) >= end) sc[a][n][e] = -INFINITY;
+          for (int e = 0; e < 4; ++e)
+            if (pos0 + n * 8 + 2 * t4 + (e & 1) >= end) sc[a][n][e] = -INFINITY;
         }
         mx0 = fmaxf(mx0, fmaxf(sc[a][n][0], sc[a][n][1]));
         mx1 = fmaxf(mx1, fmaxf(sc[a][n][2], sc[a][n][3]));
@@ -233,26 +247,39 @@ VK_DEV void attend(const Source<T>& s, uint32_t ring, int begin, int end, int fi
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
       }
-      const float mn0 = fmaxf(m[a][0], mx0), mn1 = fmaxf(m[a][1], mx1);
+      mx0 *= scale_log2;
+      mx1 *= scale_log2;
+      // the reference maximum follows only when it is passed by more than 2^8: probabilities up to 256 round as well, and most
+      // tiles need no rescaling
+      const float mn0 = mx0 > m[a][0] + 8.f || m[a][0] == -INFINITY ? mx0 : m[a][0];
+      const float mn1 = mx1 > m[a][1] + 8.f || m[a][1] == -INFINITY ? mx1 : m[a][1];
       const float mu0 = mn0 == -INFINITY ? 0.f : mn0, mu1 = mn1 == -INFINITY ? 0.f : mn1;
-      const float f0 = fast_exp2(m[a][0] - mu0), f1 = fast_exp2(m[a][1] - mu1);
-      m[a][0] = mn0;
-      m[a][1] = mn1;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        pr[a][n][0] = pack_p<T>(fast_exp2(sc[a][n][0] - mu0), fast_exp2(sc[a][n][1] - mu0), &s0);
-        pr[a][n][1] = pack_p<T>(fast_exp2(sc[a][n][2] - mu1), fast_exp2(sc[a][n][3] - mu1), &s1);
+        const float p0 = fast_exp2(fmaf(sc[a][n][0], scale_log2, -mu0)), p1 = fast_exp2(fmaf(sc[a][n][1], scale_log2, -mu0));
+        const float p2 = fast_exp2(fmaf(sc[a][n][2], scale_log2, -mu1)), p3 = fast_exp2(fmaf(sc[a][n][3], scale_log2, -mu1));
+        s0 += p0 + p1;
+        s1 += p2 + p3;
+        pr[a][n][0] = pack2<T>(p0, p1);
+        pr[a][n][1] = pack2<T>(p2, p3);
       }
-      l[a][0] = l[a][0] * f0 + s0;
-      l[a][1] = l[a][1] * f1 + s1;
+      if (__any_sync(0xffffffffu, mn0 != m[a][0] || mn1 != m[a][1])) {
+        const float f0 = fast_exp2(m[a][0] - mu0), f1 = fast_exp2(m[a][1] - mu1);
+        l[a][0] *= f0;
+        l[a][1] *= f1;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[a][i][0] *= f0;
-        o[a][i][1] *= f0;
-        o[a][i][2] *= f1;
-        o[a][i][3] *= f1;
+        for (int i = 0; i < D / 8; ++i) {
+          o[a][i][0] *= f0;
+          o[a][i][1] *= f0;
+          o[a][i][2] *= f1;
+          o[a][i][3] *= f1;
+        }
+        m[a][0] = mn0;
+        m[a][1] = mn1;
       }
+      l[a][0] += s0;
+      l[a][1] += s1;
     }
     // ---- O += P V ----
 #pragma unroll
@@ -429,7 +456,8 @@ VK_DEV void tail_item(const Args& a, const Plan& pl, uint8_t* smem) {
   const int tile = item % pl.tail_tiles;
   item /= pl.tail_tiles;
   const int kvh = item % a.HK, b = item / a.HK;
-  if (b >= a.offsets[a.P]) return;  // behind the last group
+  const int rows = a.offsets[a.P], length = a.tail_lens[b];
+  if (b >= rows) return;  // behind the last group
   Source<T> s{};
   s.k = static_cast<const T*>(a.k_pages) + kvh * D;
   s.v = static_cast<const T*>(a.v_pages) + kvh * D;
@@ -438,14 +466,14 @@ VK_DEV void tail_item(const Args& a, const Plan& pl, uint8_t* smem) {
   s.stride_page = a.stride_pp;
   s.page_shift = a.page_shift;
   s.n_pages = a.n_pages;
-  const int len = checked_len(a.tail_lens[b], a.max_pages << a.page_shift), begin = split * pl.tail_chunk;
+  const int len = checked_len(length, a.max_pages << a.page_shift), begin = split * pl.tail_chunk;
   run_item<T, D, 1, WT, true>(a, pl, smem, s, pl.prefix_splits + split, begin, min(begin + pl.tail_chunk, len), b, kvh, r,
                               tile * 16, min(tile * 16 + 16, r));
 }
 
 // MT: 16-row tiles of a prefix item.  WT: warps of a tail item.
 template <typename T, int D, int MT, int WT>
-__global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
+__global__ void __launch_bounds__(kThreads, D == 64 && MT == 1 ? 4 : 3) split_kernel(Args a, Plan pl) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Rows found;
   // Tails do not read what wide_kernel writes, and wide_kernel lets this one start only after its own wait for what came
@@ -480,7 +508,9 @@ __global__ void __launch_bounds__(kThreads) split_kernel(Args a, Plan pl) {
 //
 // A batch of MMAs takes some 600 cycles more from issue to completion than its work (256 cycles), so nothing a stream's softmax
 // waits for may hang on its last result: the scores of tile c + 1 are issued as soon as those of c are in registers, and P
-// has a place of its own, twice.  @@WIDE@@
+// has a place of its own, twice.  A tile takes some 1700 cycles, the exponentials of both streams (768 of them on their pipe)
+// and the steps around them; its MMAs take 1024.  256 rows of 32 heads on 32768 positions, D 128, fp16: 143 us, 970 TFLOP/s.
+// (P over the scores, in two buffers: 151 us; one buffer of 128 positions, MMAs issued behind a branch on the lane: 181 us.)
 template <int D>
 struct Wide {
   static constexpr int kThreads = 352;
@@ -502,18 +532,6 @@ struct Wide {
 VK_DEV uint64_t sdesc_tile(uint32_t saddr, uint32_t across) {
   constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride, descriptor version, swizzle
   return static_cast<uint64_t>(hi) << 32 | (saddr >> 4) | (across >> 4) << 16;
-}
-
-template <typename T>
-VK_DEV uint32_t pack2(float x, float y);
-template <>
-VK_DEV uint32_t pack2<__nv_bfloat16>(float x, float y) {
-  return pack_bf16x2(x, y);
-}
-template <>
-VK_DEV uint32_t pack2<__half>(float x, float y) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Largest of three, NaN if one is.
@@ -771,7 +789,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float2 t = __ffma2_rn(make_float2(v[c0 + i], v[c0 + i + 1]), sc2, nm2);
-          const float2 p = (VK_POLY >> (i >> 1 & 7)) & 1 ? poly_exp2(t) : make_float2(fast_exp2(t.x), fast_exp2(t.y));
+          const bool poly = i % 8 == 2;  // every fourth pair (none: 160 us, every fourth 153 us, every other one 164 us)
+          const float2 p = poly ? poly_exp2(t) : make_float2(fast_exp2(t.x), fast_exp2(t.y));
           rs4[(i >> 1) & 3] = __fadd2_rn(rs4[(i >> 1) & 3], p);
           pk[i / 2] = pack2<T>(p.x, p.y);
         }

@@ -25,8 +25,10 @@ static int g_pdl = 1;
 
 // Per-device record of kernels whose dynamic shared-memory limit has been raised.  The first launch of each
 // kernel on a device must happen outside stream capture (engines warm up eagerly before capturing).
+// most_shared: the SM keeps as much of its memory as shared memory as it can while the kernel runs (the default division holds
+// two CTAs of 48 KB, not four).
 template <typename K>
-static bool ensure_smem(K kernel, int bytes) {
+static bool ensure_smem(K kernel, int bytes, bool most_shared = false) {
   struct Entry {
     const void* fn;
     uint64_t mask;
@@ -42,6 +44,9 @@ static bool ensure_smem(K kernel, int bytes) {
     if (table[i].fn == fn) break;
   if (i < used && (table[i].mask & bit)) return true;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (most_shared && cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                          cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+    return false;
   if (i == used) {
     if (used == 64) return true;
     table[used++] = Entry{fn, 0};
@@ -888,22 +893,23 @@ int vk_scatter_embed(void* x, const int64_t* rows, int64_t n, int64_t x_rows, co
 
 namespace vk {
 // Splits of an axis of `most` positions among `items` independent pieces of work: as many as fill the resident CTAs (four per
-// SM) twice, chunks no shorter than `shortest` and no longer than 2048 positions.
+// SM) once, chunks of `shortest` to 4096 positions.  (256 groups of 4 rows, prefixes to 2049, tails to 1100: 81 us; filling
+// them twice 83 us, four times with chunks to 1024 89 us, chunks to 512 102 us: every split's result passes through memory.)
 static int splits_of(int most, int64_t items, int shortest, int64_t ctas) {
   if (most <= 0) return 0;
-  const int64_t want = (2 * ctas + items - 1) / items, top = (most + shortest - 1) / shortest, low = (most + 2047) / 2048;
+  const int64_t want = (ctas + items - 1) / items, top = (most + shortest - 1) / shortest, low = (most + 4095) / 4096;
   return static_cast<int>(std::max(low, std::min(want, top)));
 }
 static int chunk_of(int most, int splits) { return splits ? ((most + splits - 1) / splits + 31) / 32 * 32 : 32; }
 
 // Splits of wide_kernel's prefixes: the number that finishes first on `sms` CTAs at a time, counted in tiles of 128 positions;
-// an item costs three more than its tiles (pipeline fill, partial results).
+// an item costs six more than its tiles (pipeline fill, partial results: some 12 us).
 static int wide_splits(int64_t items, int S, int sms) {
   const int64_t tiles = (S + 127) / 128;
   int64_t best = 0;
   int at = 1;
   for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
-    const int64_t cost = (items * s + sms - 1) / sms * ((tiles + s - 1) / s + 3);
+    const int64_t cost = (items * s + sms - 1) / sms * ((tiles + s - 1) / s + 6);
     if (s == 1 || cost < best) {
       best = cost;
       at = static_cast<int>(s);
@@ -922,7 +928,7 @@ static SharedPlan shared_plan(int B, int H, int HK, int D, int P, int S, int max
   SharedPlan r;
   memset(&r, 0, sizeof(r));
   const int64_t ratio = H / HK, rows = B * ratio, ctas = 4 * 148;
-  r.wide = rows > 32 * static_cast<int64_t>(P);
+  r.wide = rows > (D == 64 ? 32 : 16) * static_cast<int64_t>(P);
   if (r.wide) {
     r.p.prefix_tiles = static_cast<int>(P + rows / 256);
     r.p.prefix_splits = wide_splits(std::max<int64_t>(P, (rows + 255) / 256) * HK, S, 148);
@@ -947,7 +953,7 @@ template <typename T, int D, int MT, int WT>
 static int shared_split(const sattn::Args& a, const sattn::Plan& p, unsigned grid, void* stream) {
   auto kern = sattn::split_kernel<T, D, MT, WT>;
   const int smem = std::max(sattn::Tile<D>::kSmem, 4 * 16 * MT * (D + 2) * 4);
-  if (!ensure_smem(kern, smem)) return VK_ERR_CUDA;
+  if (!ensure_smem(kern, smem, true)) return VK_ERR_CUDA;
   return launch(kern, dim3(grid), dim3(sattn::kThreads), smem, stream, 1, a, p);
 }
 
@@ -973,8 +979,9 @@ static int shared_run(const sattn::Args& a, SharedPlan r, void* stream) {
   }
   r.p.prefix_items = static_cast<int>(r.prefix_items);
   const unsigned n = static_cast<unsigned>(r.prefix_items + tails);
+  constexpr int MT2 = D == 64 ? 2 : 1;  // (two 16-row tiles of 128 columns do not fit the registers)
   if (rc == VK_OK && n)
-    rc = r.mt == 2 ? (r.wt == 1 ? shared_split<T, D, 2, 1>(a, r.p, n, stream) : shared_split<T, D, 2, 4>(a, r.p, n, stream))
+    rc = r.mt == 2 ? (r.wt == 1 ? shared_split<T, D, MT2, 1>(a, r.p, n, stream) : shared_split<T, D, MT2, 4>(a, r.p, n, stream))
                    : (r.wt == 1 ? shared_split<T, D, 1, 1>(a, r.p, n, stream) : shared_split<T, D, 1, 4>(a, r.p, n, stream));
   if (rc != VK_OK) return rc;
   const int splits = r.p.prefix_splits + r.p.tail_splits;
