@@ -240,6 +240,21 @@ def test_attention_same_bits_again():
         assert torch.equal(first, shared_prefix_attention(*a.args()))
 
 
+@pytest.mark.parametrize("heads", [(6, 3, 128), (8, 2, 64)])
+@pytest.mark.parametrize("each", [19, 70])
+def test_attention_same_bits_under_load(heads, each):
+    """Many groups with prefixes of many tiles, so that the loads of one tile may come long after those of later ones."""
+    from viktor_b200.ops import shared_prefix_attention
+    rs = np.random.RandomState(each)
+    sizes = rs.randint(0, 2 * each, 86)
+    a = Attend(22, HF, heads, list(sizes), list(rs.randint(0, 4500, 86)), rs.randint(0, 17, sizes.sum()), 64, nonsense=False)
+    a.check()
+    first, lse = shared_prefix_attention(*a.args(), return_lse=True)
+    for _ in range(60):
+        got = [shared_prefix_attention(*a.args(), return_lse=True) for _ in range(10)]
+        assert all(torch.equal(o, first) and torch.equal(l, lse) for o, l in got)
+
+
 def test_attention_streams_and_graphs():
     """Two calls at once on two streams, and a captured call replayed with other lengths."""
     from viktor_b200.ops import shared_prefix_attention

@@ -519,7 +519,11 @@ struct Wide {
   static constexpr int kUnit = kPos * D * 2;            // bytes of a K or V tile
   static constexpr int kSub = kPos * 128;               // bytes of 64 of its columns
   static constexpr int kQ = kRows * D * 2;              // bytes of a stream's queries
-  static constexpr int kUnits = D == 128 ? 10 : 16;
+  // A multiple of four: then a unit of the ring always holds tiles of the same one of two streams that take turns, and the stream
+  // sees every phase of its barrier.  (A barrier's parity tells a phase from the next, not from the one after: with ten units a
+  // stream saw every other phase, and took a tile whose predecessor was late in coming for its own.)
+  static constexpr int kUnits = D == 128 ? 8 : 16;
+  static_assert(kUnits % 4 == 0, "tiles of one stream in one unit of the ring");
   static constexpr int kRing = 2 * kQ;                  // behind the queries
   static constexpr int kBars = kRing + kUnits * kUnit;
   static constexpr int kSmem = kBars + 512 + 1024;
@@ -921,7 +925,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) join_kernel(Args a, Pla
   for (int i = 0; i < PER; ++i) o[i] = 0.f;
   for (int s0 = warp * 32; s0 < splits; s0 += W * 32) {
     const int n = min(32, splits - s0);
-    const float2 ml = lane < n ? pl.ws_ml[(s0 + lane) * rows + row] : make_float2(-INFINITY, 0.f);
+    const float2 ml = lane < n ? __ldcg(&pl.ws_ml[(s0 + lane) * rows + row]) : make_float2(-INFINITY, 0.f);
     float mn = ml.x;
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
