@@ -37,11 +37,11 @@ def attend_bounds(out, spread, span, n, D, dtype):
 
     Scores: products of two 16-bit values are exact in float32; D of them are summed, so a score is off by at most
     (D + 2) 2^-23 span, and times log2(e), minus the maximum (|z| <= span): another 4 2^-24 span.  exp2 is off by 2^-21
-    relative.  So every p is off by delta = (D + 4) 2^-23 span + 2^-21 relative, and the sum of them by no more.  Only the product
-    with V takes p rounded
-    to the type (u): 2 (delta + u) at most for p_j / sum p; the log of the sum is off by delta, and 2^-20 for the joins and the log.  The n products are summed in chains
-    of at most n / 16 + 64 float32 additions (a matrix instruction takes 16 positions at least one at a time: n / 16 + 16
-    steps, then the joins), (n / 16 + 64) 2^-23 of spread, twice (values and sum).  The result is rounded once: u |out|."""
+    relative.  So every p is off by delta = (D + 4) 2^-23 span + 2^-21 relative, and the sum of them by no more.  Only the
+    product with V takes p rounded to the type (u): 2 (delta + u) at most for p_j / sum p; the log of the sum is off by delta,
+    and 2^-20 for the joins and the log.  The n products are summed in chains of at most n / 16 + 64 float32 additions (a
+    matrix instruction takes 16 positions at least one at a time: n / 16 + 16 steps, then the joins), (n / 16 + 64) 2^-23 of
+    spread, twice (values and sum).  The result is rounded once: u |out|."""
     u = torch.finfo(dtype).eps / 2
     delta = (D + 4) * 2.0 ** -23 * span + 2.0 ** -21
     chain = 2 * (n / 16 + 64) * 2.0 ** -23

@@ -4,6 +4,13 @@
 //   out[b, h, :] = sum_j p_j v_j,  p = softmax_j(scale * q[b, h] . k_j),  j in prefix(g) then tail(b),  KV head h / (H / HK)
 //
 // A row with nothing to attend gives 0 (lse -inf); rows behind the last group are not touched.
+//
+// Prefix and tails are split over CTAs, each with a running maximum and sum (base 2); a last kernel joins the partial results,
+// in a fixed order, so equal calls give equal bits and nothing in the workspace outlives a call.
+//  * few rows of a group and KV head (up to 32 of D 64, 16 of D 128 on average), and every tail: split_kernel, on the warp tensor
+//    cores, bound by HBM.  256 groups of 4 rows, prefixes to 2049, tails to 1100 (451 MB): 75 us, 6.0 TB/s.  4 rows x 16 heads
+//    on 131071 positions (537 MB): 88 us, 6.1 TB/s.
+//  * more rows: wide_kernel, on the 5th-generation tensor cores, bound by the exponentials and the steps around them.
 #pragma once
 
 #include <type_traits>
@@ -509,8 +516,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 && MT == 1 ? 4 : 3) split_ke
 // A batch of MMAs takes some 600 cycles more from issue to completion than its work (256 cycles), so nothing a stream's softmax
 // waits for may hang on its last result: the scores of tile c + 1 are issued as soon as those of c are in registers, and P
 // has a place of its own, twice.  A tile takes some 1700 cycles, the exponentials of both streams (768 of them on their pipe)
-// and the steps around them; its MMAs take 1024.  256 rows of 32 heads on 32768 positions, D 128, fp16: 143 us, 970 TFLOP/s.
-// (P over the scores, in two buffers: 151 us; one buffer of 128 positions, MMAs issued behind a branch on the lane: 181 us.)
+// and the steps around them; its MMAs take 1024.  256 rows of 32 heads on 32768 positions, D 128, fp16: 147 us, 940 TFLOP/s.
+// (P over the scores, in two buffers, which hung on the last result: 5 % more; one buffer of 128 positions and MMAs issued behind a
+// branch on the lane: 181 us.)
 template <int D>
 struct Wide {
   static constexpr int kThreads = 352;

@@ -354,7 +354,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k
 
     Returns out [B, H, D], with return_lse also the log of the sum of exponentials [B, H] (float32).  A row with nothing
     to attend gets 0 and -inf; rows behind the last group are not written.  What a cache holds behind a length is not
-    used.  workspace: uint8, vk_shared_attention_workspace_bytes; calls that may run at the same time need one each (by
+    used.  No gradients.  workspace: uint8, vk_shared_attention_workspace_bytes; calls that may run at the same time need one each (by
     default every call allocates its own)."""
     q_shape, prefix_shape, pages_shape, table_shape = q.shape, k_prefix.shape, k_pages.shape, page_table.shape
     _need(len(q_shape) == 3 and len(prefix_shape) == len(pages_shape) == 4 and len(table_shape) == 2,
@@ -505,7 +505,8 @@ def pages_free(pages: KVPages, rows=None):
 
 def pages_compact(pages: KVPages):
     """Moves the pages in use to the lowest numbers: those at or above their count go into the free ones below it, both in
-    ascending order.  Returns the count, int32 [1] on the device."""
+    ascending order; table and refs follow.  (A page that only refs names, not the table, is moved as well.)  Returns the
+    count, int32 [1] on the device."""
     live = torch.empty(1, dtype=_I32, device=pages.device)
     ws = pages._workspace(0)
     table, _, refs, rows, max_pages, n_pages = pages._books()
