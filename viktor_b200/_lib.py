@@ -76,7 +76,7 @@ _lib = None
 _HOST_ONLY = {"vk_version", "vk_read_device_errors", "vk_set_pdl", "vk_decode_attention_workspace_bytes",
               "vk_decode_attention_i8_workspace_bytes", "vk_align", "vk_overlap_cut", "vk_stitch",
               "vk_shared_attention_workspace_bytes", "vk_pages_workspace_bytes"}
-_KERNELS = {"vk_shared_attention": 2, "vk_pages_fork": 2, "vk_pages_compact": 2}  # kernels of one call where it is not one
+_KERNELS = {"vk_shared_attention": 2, "vk_pages_fork": 2, "vk_pages_compact": 2}  # at least, where a call launches more than one
 launches = 0  # kernels launched through call()
 
 

@@ -636,7 +636,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
-      for (int u = 0; u < 2 * tiles; ++u) {
+      int u = 0;
+      for (; u < 2 * tiles; ++u) {
         const int slot = u % W::kUnits;
         if (u >= W::kUnits && !mbar_wait(&u_empty[slot], ((u / W::kUnits) & 1) ^ 1)) {
           raise_error(ERR_WAIT_EMPTY);
@@ -649,6 +650,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         for (int c = 0; c < D / 64; ++c)
           tma_load_4d(to + c * W::kSub, map, &u_full[slot], c * 64, w.kvh, begin + (u >> 1) * W::kPos, w.g);
       }
+      // no load may be under way when the CTA ends, whatever the other warps have given up on
+      for (int i = u > W::kUnits ? u - W::kUnits : 0; i < u; ++i)
+        if (!mbar_wait(&u_full[i % W::kUnits], (i / W::kUnits) & 1)) raise_error(ERR_WAIT_FULL);
     }
   } else if (warp == 1 || warp == 10) {
     // ---------------- MMA issue of one stream: the whole warp in step, one lane issues ----------------
