@@ -98,6 +98,7 @@ VK_DEV int row_len(const Pool& p, int row) {
   raise_error(ERR_BOUNDS);
   return len < 0 ? 0 : most;
 }
+// Of a length a row can have: at most max_pages whole pages, so the sum stays below 2^31.
 VK_DEV int pages_of(const Pool& p, int len) { return (len + (1 << p.page_shift) - 1) >> p.page_shift; }
 
 struct ExtendArgs {
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(ExtendArgs a, bool
       if (ok) {
         const int len = row_len(p, row);
         a.len[i] = len;
-        ok = len + a.count <= p.max_pages << p.page_shift;
+        ok = a.count <= (p.max_pages << p.page_shift) - len;  // (their sum may pass 2^31)
         if (ok) need = pages_of(p, len + a.count) - pages_of(p, len);
       }
       if (!ok) raise_error(ERR_BOUNDS);
