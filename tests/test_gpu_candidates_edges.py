@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_candidates import BF, I32, errors, i32
+from test_gpu_candidates import BF, I32, Attend, errors, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -14,6 +14,25 @@ def _errors_clear():
     yield
     torch.cuda.synchronize()
     check_device_errors()
+
+
+# ------------------------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("heads,B,P,lo", [((1, 1, 64), 180, 6, 60), ((1, 1, 64), 1000, 3, 100), ((2, 1, 128), 40, 6, 8),
+                                          ((2, 1, 128), 500, 3, 50)])
+def test_attention_offsets_that_descend(heads, B, P, lo):
+    """Offsets 0, B, lo, B, ...: the second group is refused, the first and the third have rows and tiles in common.  That is
+    reported, rows below lo are right, and nothing is written behind the workspace."""
+    from viktor_b200._lib import load
+    from viktor_b200.ops import shared_prefix_attention
+    a = Attend(30, BF, heads, [B] + [0] * (P - 1), [300, 70, 150, 4, 5, 6][:P], [b % 4 for b in range(B)], 16)
+    n = load().vk_shared_attention_workspace_bytes(B, *heads, P, 300, a.table.shape[1] * 16)
+    ws = torch.full((n + (1 << 20),), 255, dtype=torch.uint8, device="cuda")
+    want = shared_prefix_attention(*a.args(), workspace=ws)
+    assert errors() == 0 and bool((ws[n:] == 255).all())
+    a.offsets[2] = lo
+    for _ in range(20):
+        got = shared_prefix_attention(*a.args(), workspace=ws)
+        assert errors() == 8 and torch.equal(got[:lo], want[:lo]) and bool((ws[n:] == 255).all())
 
 
 # ------------------------------------------------------------------------------------------------ pages

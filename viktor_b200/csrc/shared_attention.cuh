@@ -425,16 +425,22 @@ VK_DEV void run_item(const Args& a, const Plan& pl, uint8_t* smem, const Source<
 struct Rows {
   int g, b0, len, kvh, split, x0, x1;
 };
-// The item of this CTA of `threads` threads with tiles of kRows rows; found: shared.  Every thread looks at its groups; the one
-// whose group's tiles hold this one (group g's begin at floor(offset_g * r / kRows) + g) says so: one round of loads.
+// The item of this CTA of `threads` threads with tiles of kRows rows; found: shared.  Every thread looks at every threads-th
+// group (one round of loads for up to `threads` groups); the one whose group's tiles hold this one (group g's begin at
+// floor(offset_g * r / kRows) + g) says so.  Offsets that do not ascend can give a tile to several groups: the first thread
+// to say so has it, so that the record is always of one group, whose rows lie in 0 .. B - 1.
 template <int kRows, int threads>
 VK_DEV Rows find_rows(const Args& a, const Plan& pl, Rows* found) {
+  constexpr int kNone = 0x7fffffff;
   const int r = a.H / a.HK;
   int item = blockIdx.x;
   const int split = item % pl.prefix_splits;
   item /= pl.prefix_splits;
   const int kvh = item % a.HK, tile = item / a.HK;
-  if (threadIdx.x == 0) found->x0 = found->x1 = 0;
+  if (threadIdx.x == 0) {
+    found->x0 = kNone;
+    found->x1 = 0;
+  }
   __syncthreads();
   for (int g = threadIdx.x; g < a.P; g += threads) {
     const int lo = a.offsets[g], hi = a.offsets[g + 1], length = a.prefix_lens[g];
@@ -445,8 +451,13 @@ VK_DEV Rows find_rows(const Args& a, const Plan& pl, Rows* found) {
     const int first = static_cast<int>(static_cast<int64_t>(lo) * r / kRows) + g;
     const int64_t x0 = static_cast<int64_t>(tile - first) * kRows, all = static_cast<int64_t>(hi - lo) * r;
     if (x0 < 0 || x0 >= all) continue;
-    const int len = checked_len(length, a.S);
-    *found = Rows{g, lo, len, kvh, split, static_cast<int>(x0), static_cast<int>(x0 + kRows < all ? x0 + kRows : all)};
+    if (atomicCAS(&found->x0, kNone, static_cast<int>(x0)) != kNone) continue;
+    found->x1 = static_cast<int>(x0 + kRows < all ? x0 + kRows : all);
+    found->g = g;
+    found->b0 = lo;
+    found->len = checked_len(length, a.S);
+    found->kvh = kvh;
+    found->split = split;
   }
   __syncthreads();
   return *found;
