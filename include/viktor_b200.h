@@ -285,7 +285,7 @@ size_t vk_shared_attention_workspace_bytes(int B, int H, int HK, int D, int P, i
  * kvh * D + d, p < S, strides multiples of 8 (one layer of a static cache whose rows are the prefixes).  k_pages /
  * v_pages: n_pages pages of `page` tokens (a power of two, 8..256), element (page, slot, kvh, d) at page * stride_pp +
  * (slot * HK + kvh) * D + d; page_table [B, max_pages] i32 (row stride stride_table) names row b's pages.
- * prefix_lens [P], group_offsets [P + 1] (ascending from 0, at most B), tail_lens [B] i32.  lse [B, H] f32 (log of the sum of
+ * S + max_pages * page at most 2^31 - 2^16.  prefix_lens [P], group_offsets [P + 1] (ascending from 0, at most B), tail_lens [B] i32.  lse [B, H] f32 (log of the sum of
  * exponentials) or NULL.  A row with nothing to attend gets 0 and lse -inf; rows behind the last group are left as they
  * were.  What lies behind a prefix's or a tail's length is not used, whatever it holds.  Lengths, offsets and pages out
  * of range are reported in the device error word (results of those rows are unspecified).  out must not overlap q. */

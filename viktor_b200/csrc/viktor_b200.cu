@@ -918,6 +918,10 @@ static int wide_splits(int64_t items, int S, int sms) {
   return at;
 }
 
+// Positions of a prefix and a tail together.  Chunks end less than 2^15 behind them (64 splits of wide_kernel are rounded up to 128
+// positions, some 600 of split_kernel to 32, or chunks have 4096) and loads look a few tiles further: all below 2^31.
+constexpr int64_t kMostPositions = (int64_t(1) << 31) - (1 << 16);
+
 struct SharedPlan {
   bool wide;
   int mt, wt;
@@ -1022,7 +1026,9 @@ static int penalize_run(const logit::Args& a, void* stream) {
 extern "C" {
 
 size_t vk_shared_attention_workspace_bytes(int B, int H, int HK, int D, int P, int S, int max_tail) {
-  if (B <= 0 || H <= 0 || HK <= 0 || H % HK || D <= 0 || P <= 0 || S <= 0 || max_tail < 0) return 0;
+  if (B <= 0 || H <= 0 || HK <= 0 || H % HK || D <= 0 || P <= 0 || S <= 0 || max_tail < 0 ||
+      static_cast<int64_t>(S) + max_tail > kMostPositions)
+    return 0;
   const SharedPlan r = shared_plan(B, H, HK, D, P, S, max_tail);
   return static_cast<size_t>(r.p.prefix_splits + r.p.tail_splits) * B * H * (D + 2) * 4;
 }
@@ -1042,7 +1048,7 @@ int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* 
       !workspace || (max_pages && !page_table))
     return VK_ERR_ARG;
   const int64_t token = static_cast<int64_t>(HK) * D, cap = int64_t(1) << 31;
-  if (static_cast<int64_t>(B) * H >= cap || static_cast<int64_t>(max_pages) * page + S >= cap ||
+  if (static_cast<int64_t>(B) * H >= cap || static_cast<int64_t>(max_pages) * page + S > kMostPositions ||
       stride_q < static_cast<int64_t>(H) * D || stride_q % 8 || stride_ks < token || stride_ks % 8 ||
       stride_kb < stride_ks * S || stride_kb % 8 || stride_pp < token * page || stride_pp % 8 ||
       stride_table < max_pages)

@@ -295,6 +295,7 @@ def scatter_embed(x, rows, emb, token):
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _I32 = torch.int32
 _PAGES = (8, 16, 32, 64, 128, 256)
+_MOST_POSITIONS = (1 << 31) - (1 << 16)
 
 
 def _launch(name, device, *args):
@@ -350,7 +351,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k
     q [B, H, D] bf16 or fp16 (D 64 or 128); k_prefix / v_prefix [P, S, HK, D]: one layer of a static cache, one row per
     group; prefix_lens [P] int32; group_offsets [P + 1] int32: rows group_offsets[g] .. group_offsets[g + 1] - 1 belong
     to group g.  k_pages / v_pages [n_pages, page, HK, D]: one layer of a KVPages; page_table [B, max_pages] int32;
-    tail_lens [B] int32.  Query head h reads KV head h // (H // HK).  scale: 1 / sqrt(D) by default.
+    tail_lens [B] int32; S + max_pages * page at most 2^31 - 2^16.  Query head h reads KV head h // (H // HK).  scale: 1 / sqrt(D) by default.
 
     Returns out [B, H, D], with return_lse also the log of the sum of exponentials [B, H] (float32).  A row with nothing
     to attend gets 0 and -inf; rows behind the last group are not written.  What a cache holds behind a length is not
@@ -370,6 +371,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, prefix_lens, group_offsets, k
     _need(D == 64 or D == 128, "head_dim must be 64 or 128")
     _need(P > 0 and S > 0 and HK > 0 and n_pages > 0 and H > 0 and H % HK == 0, "empty cache, or heads that do not divide")
     _need(page in _PAGES, "pages hold a power of two from 8 to 256 tokens")
+    _need(S + max_pages * page <= _MOST_POSITIONS, "S + max_pages * page must be at most 2^31 - 2^16")
     _need(v_prefix.shape == prefix_shape and prefix_shape[3] == D, "k_prefix and v_prefix: [P, S, HK, D]")
     _need(v_pages.shape == pages_shape and pages_shape[2] == HK and pages_shape[3] == D, "k_pages and v_pages: [n_pages, page, "
           "HK, D]")
