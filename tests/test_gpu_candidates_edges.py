@@ -1,9 +1,12 @@
 """The operators that decode several candidates of a chunk at the ends of what their entry points accept."""
 
+import math
+
 import pytest
 import torch
 
-from test_gpu_candidates import BF, I32, Attend, errors, i32
+from candidates_ref import attend_bounds, attend_ref
+from test_gpu_candidates import BF, HF, I32, INF, Attend, errors, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -17,6 +20,89 @@ def _errors_clear():
 
 
 # ------------------------------------------------------------------------------------------------ attention
+def check_attend(a):
+    """As Attend.check, with the bound on the rounding of fp16 probabilities completed: one that is below 2^-14 next to its
+    reference is not off by u relative but by up to 2^-25, half the step of the smallest fp16 values.  The reference of a chunk is at
+    least 11 (base 2) below its largest score, so the sum of all probabilities is at least 2^11 there, and every position adds at
+    most 2^-36 |v_j|."""
+    from viktor_b200.ops import shared_prefix_attention
+    out = torch.full(a.q.shape, 7.0, dtype=a.q.dtype, device="cuda")
+    got, lse = shared_prefix_attention(*a.args(), out=out, return_lse=True)
+    n, D, dtype = a.q.shape[0] - a.pad, a.q.shape[2], a.q.dtype
+    want, want_lse, spread, span = attend_ref(*a.args())
+    tol, tol_lse = attend_bounds(want, spread, span, a.most, D, dtype)
+    if dtype is HF:
+        largest = max(float(torch.nan_to_num(x.float(), nan=0.0).abs().max()) for x in (a.v, a.vp))
+        tol = tol + 2.0 ** -36 * a.most * largest
+    err = (got.double() - want).abs()
+    assert bool((err <= tol)[:n].all()), f"out off by up to {float((err / tol)[:n].max()):.3g} of the bound"
+    empty = want_lse[:n] == -INF
+    assert bool((lse[:n] == -INF)[empty].all()) and bool((got[:n][empty] == 0).all())
+    e = (lse[:n].double() - want_lse[:n]).abs()[~empty]
+    assert bool((e <= tol_lse[:n][~empty] + 2.0 ** -22 * want_lse[:n][~empty].abs()).all()), f"lse off by {float(e.max()):.3g}"
+    assert bool((got[n:] == 7.0).all()), "rows behind the last group were written"
+
+
+# few rows of each group; more than 32 of a KV head; more than 128
+FORMS = [((2, 1, 64), [1] * 300), ((2, 1, 128), [1] * 300), ((40, 1, 64), [1] * 148), ((40, 1, 128), [1] * 148), ((40, 1, 64), [4] * 148),
+         ((40, 1, 128), [4] * 148)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,sizes", FORMS)
+@pytest.mark.parametrize("gap", [13.0, 20.6, 25.05, 27.5])
+def test_attention_dominant_positions_of_small_value(dtype, heads, sizes, gap):
+    """A few positions whose scores are 2^gap above all others, with values of 0: what the others add up to is not lost.  They
+    stand where every warp and stream that goes through a prefix meets one first."""
+    D = heads[2]
+    a = Attend(31, dtype, heads, sizes, [700 - g % 7 for g in range(len(sizes))], [5] * sum(sizes), 16)
+    a.q *= 0.05
+    a.k[..., 0] = a.kp[..., 0] = 0.0
+    a.q[..., 0] = 4.0
+    for x in (a.v, a.vp):
+        x.mul_(0.1).add_(1.0).mul_(64.0)
+    for at in (0, 16, 32, 48, 64, 96):
+        a.k[:, at, :, 0] = gap * math.log(2.0) * math.sqrt(D) / 4.0
+        a.v[:, at] = 0.0
+    check_attend(a)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("page", [8, 64])
+@pytest.mark.parametrize("heads,rows", [((8, 2, 64), 7), ((2, 1, 128), 2500)])
+def test_attention_dominant_positions_in_tails(dtype, page, heads, rows):
+    """The same in the tails, for few and for many rows."""
+    D = heads[2]
+    a = Attend(32, dtype, heads, [rows], [3], [200 - b % 9 for b in range(rows)], page)
+    a.q *= 0.05
+    a.k[..., 0] = a.kp[..., 0] = 0.0
+    a.q[..., 0] = 4.0
+    for x in (a.v, a.vp):
+        x.mul_(0.1).add_(1.0).mul_(64.0)
+    for at in (0, 16, 32, 48, 64, 96):
+        pages = a.table[:, at // page].long()
+        a.kp[pages, at % page, :, 0] = 21.0 * math.log(2.0) * math.sqrt(D) / 4.0
+        a.vp[pages, at % page] = 0.0
+    check_attend(a)
+
+
+@pytest.mark.parametrize("size", [1e-3, 30.0])
+def test_attention_peaked_and_flat_in_fp16(size):
+    a = Attend(33, HF, (8, 2, 64), [3, 60], [90, 700], [20] * 63, 16)
+    a.q *= size
+    check_attend(a)
+
+
+def test_attention_growing_scores_in_fp16():
+    """The running maximum rises from tile to tile, by more and by less than the reference may lag behind, and falls again."""
+    for top in (3.0, 12.0, 40.0):
+        a = Attend(34, HF, (8, 2, 64), [3, 70], [900, 900], [30] * 73, 16)
+        a.k[:, :, :, 0] = torch.linspace(-top, top, 900, device="cuda").to(HF)[None, :, None]
+        a.k[1] = a.k[1].flip(0)
+        a.q[:, :, 0] = 8
+        check_attend(a)
+
+
 @pytest.mark.parametrize("heads,B,P,lo", [((1, 1, 64), 180, 6, 60), ((1, 1, 64), 1000, 3, 100), ((2, 1, 128), 40, 6, 8),
                                           ((2, 1, 128), 500, 3, 50)])
 def test_attention_offsets_that_descend(heads, B, P, lo):

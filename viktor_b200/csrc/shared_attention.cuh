@@ -50,7 +50,7 @@ struct Plan {
   bool behind_wide;   // launched right behind wide_kernel of the same call
   float scale_log2;
   float* ws_o;        // [prefix_splits + tail_splits][B * H][D]
-  float2* ws_ml;      // [prefix_splits + tail_splits][B * H]: maximum (of scores in base 2) and sum
+  float2* ws_ml;      // [prefix_splits + tail_splits][B * H]: reference (below, of scores in base 2) and sum
 };
 
 template <typename T>
@@ -80,6 +80,18 @@ VK_DEV uint32_t pack2<__half>(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+
+// Probabilities are taken relative to a reference: the largest score so far (base 2) less kDrop, followed only when that is passed by
+// more than kLag, so that most tiles need no rescaling.  They lie below 2^(kDrop + kLag) and are rounded to the type for the
+// product with V, their sum is not.  bf16 has the exponents of float32: any reference will do.  fp16 is normal down to 2^-14 and
+// ends at 2^16: with the reference 11 below the maximum a probability keeps its 11 bits down to 2^-25 of the largest, and is off
+// by at most 2^-36 of it below (with the maximum for a reference: 2^-14 and 2^-25, and next to one dominant position with a
+// small value the others were lost); a longer lag would take that room away.
+template <typename T>
+struct Ref {
+  static constexpr float kDrop = std::is_same<T, __half>::value ? 11.f : 0.f;
+  static constexpr float kLag = std::is_same<T, __half>::value ? 4.f : 8.f;
+};
 
 // 16 bytes from global to shared memory; the second form: zeros where !use.
 VK_DEV void cp_async16(uint32_t dst, const void* src) {
@@ -232,7 +244,7 @@ VK_DEV void attend(const Source<T>& s, uint32_t ring, int begin, int end, int fi
           mma_16816<T>(sc[a][n + 1], q[a][ks], b[2], b[3]);
         }
       }
-    // ---- softmax in base 2; probabilities are rounded to the type for the product below, their sum is not ----
+    // ---- softmax in base 2 ----
     const int pos0 = begin + t * kPos;
     const bool partial = pos0 + kPos > end;
     uint32_t pr[MT][kN][2];
@@ -254,12 +266,10 @@ VK_DEV void attend(const Source<T>& s, uint32_t ring, int begin, int end, int fi
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
       }
-      mx0 *= scale_log2;
-      mx1 *= scale_log2;
-      // the reference maximum follows only when it is passed by more than 2^8: probabilities up to 256 round as well, and most
-      // tiles need no rescaling
-      const float mn0 = mx0 > m[a][0] + 8.f || m[a][0] == -INFINITY ? mx0 : m[a][0];
-      const float mn1 = mx1 > m[a][1] + 8.f || m[a][1] == -INFINITY ? mx1 : m[a][1];
+      mx0 = mx0 * scale_log2 - Ref<T>::kDrop;
+      mx1 = mx1 * scale_log2 - Ref<T>::kDrop;
+      const float mn0 = mx0 > m[a][0] + Ref<T>::kLag || m[a][0] == -INFINITY ? mx0 : m[a][0];
+      const float mn1 = mx1 > m[a][1] + Ref<T>::kLag || m[a][1] == -INFINITY ? mx1 : m[a][1];
       const float mu0 = mn0 == -INFINITY ? 0.f : mn0, mu1 = mn1 == -INFINITY ? 0.f : mn1;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
@@ -564,7 +574,7 @@ VK_DEV float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// 2^x of two values, -inf..9, on the FMA pipes, for a part of the probabilities: the SM takes 16 exponentials a cycle but 128 FMAs.
+// 2^x of two values, -inf..16, on the FMA pipes, for a part of the probabilities: the SM takes 16 exponentials a cycle but 128 FMAs.
 // x is split into a whole number n (by adding 1.5 * 2^23) and f in -0.5..0.5; 2^f by the polynomial of degree 5 with the
 // smallest largest relative error on that range (fitted in float64 by reweighted least squares: 2^-23.7; in float32
 // arithmetic 2^-22.1); n goes into the exponent bits.  Below -127 the result is 2^-149.  NaN gives some number: the caller
@@ -804,9 +814,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 #pragma unroll
         for (int i = 12; i < W::kPos; i += 8) mx4[k] = i + 4 < W::kPos ? max3_nan(mx4[k], v[i + k], v[i + k + 4]) : max3_nan(mx4[k], v[i + k], v[i + k]);
       }
-      const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * pl.scale_log2;
-      // the reference maximum follows only when it is passed by more than 2^8: probabilities up to 256 round as well
-      const float m_new = mx > m + 8.f || m == -INFINITY ? fmaxf(m, mx) : m;
+      const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * pl.scale_log2 - Ref<T>::kDrop;
+      const float m_new = mx > m + Ref<T>::kLag || m == -INFINITY ? fmaxf(m, mx) : m;
       const float mu = m_new == -INFINITY ? 0.f : m_new;
       const float2 sc2 = make_float2(pl.scale_log2, pl.scale_log2), nm2 = make_float2(-mu, -mu);
       float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -992,7 +1001,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) join_kernel(Args a, Pla
   T* op = static_cast<T*>(a.out) + row * D + lane * PER;
 #pragma unroll
   for (int i = 0; i < PER; i += 2) *reinterpret_cast<uint32_t*>(op + i) = l == 0.f ? 0u : pack2<T>(o[i] / l, o[i + 1] / l);
-  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m * 0.69314718055994531f + logf(l);
+  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;  // (of one position m + log2 l is exact)
 }
 
 }  // namespace sattn
