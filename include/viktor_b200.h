@@ -313,7 +313,8 @@ int vk_pages_extend(int32_t* table, int32_t* lens, int32_t* refs, int rows, int 
 
 /* Rows dst[i] become copies of rows src[i] as they were before the call, i < n: full pages are shared, a partly filled
  * last page is copied in all layers (k, v [layers, n_pages, page, token_bytes], token_bytes a multiple of 16).  What a
- * dst row held before is released; a page released by a call is given out from the next call on. */
+ * dst row held before is released; a page released by a call is given out from the next call on.  Where the page to be
+ * copied is out of range, the dst row is not changed and that is reported (VK_DEVERR_BOUNDS). */
 int vk_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page,
                   const int32_t* src, const int32_t* dst, int n, void* k, void* v, int layers, int token_bytes,
                   void* workspace, size_t workspace_bytes, void* stream);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from candidates_ref import attend_bounds, attend_ref
-from test_gpu_candidates import BF, HF, I32, INF, Attend, errors, i32
+from test_gpu_candidates import BF, HF, I32, INF, Attend, errors, i32, pool
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,28 @@ def test_extend_rows_near_31_bits():
     places, slots = pages_extend(p, 300)
     assert places[0].tolist() == [4] * 44 + [1] * 256 and p.table[0, -2:].tolist() == [4, 1] and p.refs.tolist() == [1, 1, 0, 0, 1, 0]
     assert slots[0].tolist() == list(range(212, 256)) + list(range(256)) and errors() == 0
+
+
+@pytest.mark.parametrize("bad", [-1, -7, 40, 2 ** 31 - 1])
+@pytest.mark.parametrize("max_pages", [6, 3000])
+def test_fork_of_a_row_whose_last_page_is_out_of_range(bad, max_pages):
+    """Nothing can be copied, so the row stays as it was, and no page is spent on it; other rows are served."""
+    from viktor_b200.ops import pages_extend, pages_fork
+    p = pool(max_pages=max_pages)
+    pages_extend(p, 13, i32([0, 1, 2]))
+    p.table[0, 1] = bad
+    p.refs[1] = 0
+    before = p.table.clone(), p.lens.clone(), p.refs.clone(), p.k.clone(), p.v.clone()
+    pages_fork(p, i32([0, 2, 0]), i32([1, 3, 4]))
+    assert errors() == 8
+    table, lens, refs, k, v = before
+    table[3, :2] = i32([4, 1])  # the lowest free page is 1
+    lens[3], refs[4], refs[1] = 13, 2, 1
+    k[:, 1, :5], v[:, 1, :5] = k[:, 5, :5], v[:, 5, :5]
+    assert torch.equal(p.table, table) and torch.equal(p.lens, lens) and torch.equal(p.refs, refs)
+    assert torch.equal(p.k, k) and torch.equal(p.v, v)
+    p.table[0, 1] = 7  # repaired: served
+    p.refs[7] = 1
+    pages_fork(p, i32([0]), i32([4]))
+    assert errors() == 0 and p.table[4, :2].tolist() == [0, 6] and p.lens[4] == 13
+    assert torch.equal(p.k[:, 6, :5], p.k[:, 7, :5])

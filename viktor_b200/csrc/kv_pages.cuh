@@ -260,8 +260,16 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(ForkArgs a, bool cel
       if (!ok) raise_error(ERR_BOUNDS);
       if (ok && s == t) ok = false;
       if (ok) {
-        a.len[i] = row_len(p, s);
-        need = (a.len[i] & mask) != 0;
+        const int len = row_len(p, s);
+        a.len[i] = len;
+        if (len & mask) {  // the page to be copied
+          const int from = p.table[static_cast<int64_t>(s) * p.max_pages + (len >> p.page_shift)];
+          ok = from >= 0 && from < p.n_pages;
+          if (ok)
+            need = 1;
+          else
+            raise_error(ERR_BOUNDS);
+        }
       }
     }
     int n;
@@ -280,11 +288,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(ForkArgs a, bool cel
         raise_error(ERR_PAGES);
         a.state[i] = -1;
       } else if (part) {
-        const int from = p.table[static_cast<int64_t>(a.src[i]) * p.max_pages + full];
-        if (from >= 0 && from < p.n_pages)
-          m = Move{from, a.free_list[at], part};
-        else
-          raise_error(ERR_BOUNDS);
+        m = Move{p.table[static_cast<int64_t>(a.src[i]) * p.max_pages + full], a.free_list[at], part};
       }
     }
     a.moves[i] = m;

@@ -488,7 +488,8 @@ def pages_extend(pages: KVPages, count=1, rows=None):
 def pages_fork(pages: KVPages, src, dst):
     """Rows dst[i] (int32 [n]) become copies of rows src[i] as they were before the call.  Full pages are shared; a partly
     filled last page is copied in every layer.  What the dst rows held is released, and given out again from the next
-    call on.  src[i] == dst[i] leaves the row as it is."""
+    call on.  src[i] == dst[i] leaves the row as it is.  A row that is out of range, a dst named before, or a src whose page to be
+    copied is out of range or for which no page is left changes nothing and is reported by check_device_errors()."""
     src_ptr, n = pages._rows("src", src)
     dst_ptr, m = pages._rows("dst", dst)
     _need(src is not None and dst is not None and n == m, "src and dst must have one length")
