@@ -33,7 +33,7 @@ extern "C" {
 #define VK_DEVERR_WAIT_EMPTY 2u  /* a producer gave up waiting for a free stage */
 #define VK_DEVERR_WAIT_ACCUM 4u  /* an epilogue gave up waiting for the tensor-core accumulator */
 #define VK_DEVERR_BOUNDS 8u      /* an index (token, position, cache row) was out of range; access skipped */
-#define VK_DEVERR_PAGES 16u      /* no free cache page was left; the row it was for was not changed */
+#define VK_DEVERR_PAGES 16u      /* too few free cache pages were left; the row they were for was not changed */
 
 /* Element types of the entry points that take more than one. */
 #define VK_BF16 0
@@ -300,8 +300,9 @@ int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* 
  * tokens of each row, refs [n_pages] i32 how many rows name a page (0: free); page = tokens per page, a power of two,
  * 8..256.  All but the last page of a row are full and only full pages are shared.  Free pages are given out the lowest
  * first, in the order of the list.  Row numbers out of range, and all but the first naming of a row that a list names
- * twice, are skipped and reported (VK_DEVERR_BOUNDS); a row for which no page is left is not changed and reported
- * (VK_DEVERR_PAGES).  Calls on the same pages follow one another on one stream.
+ * twice, are skipped and reported (VK_DEVERR_BOUNDS); a row that needs more pages than the ones before it in the list
+ * have left is not changed and reported (VK_DEVERR_PAGES), and so is every later row of the call that needs a page, even
+ * if fewer would have done: no row takes a page that an earlier one lacked.  Calls on the same pages follow one another on one stream.
  * Workspace bytes the three calls below need for n listed rows (contents do not matter). */
 size_t vk_pages_workspace_bytes(int rows, int max_pages, int n_pages, int n);
 

@@ -146,6 +146,35 @@ def test_extend_rows_near_31_bits():
     assert slots[0].tolist() == list(range(212, 256)) + list(range(256)) and errors() == 0
 
 
+@pytest.mark.parametrize("rows", [4, 1000])
+def test_extend_with_too_few_pages(rows):
+    """The first row that needs more pages than are left stops every later one of the call that needs a page; rows that need
+    none are served, and what is left is there for the next call."""
+    from viktor_b200.ops import pages_extend
+    p = pool(n_pages=rows + 1, rows=rows, max_pages=4, layers=1, hk=1)
+    pages_extend(p, 3, i32(range(2, rows)))  # one page each
+    p.refs[rows - 2:] = 1
+    p.refs[rows] = 0  # one free page
+    p.lens[1], p.table[1, 0] = 7, rows - 1
+    table, lens, refs = p.table.clone(), p.lens.clone(), p.refs.clone()
+    # 9 tokens: row 0 needs two pages, the others one each
+    places, slots = pages_extend(p, 9)
+    assert errors() == 16 and bool((places == -1).all()) and bool((slots == -1).all())
+    assert torch.equal(p.table, table) and torch.equal(p.lens, lens) and torch.equal(p.refs, refs)
+    # 5 tokens: rows 0 and 1 need one page each, and row 0 gets it; the others have room
+    places, slots = pages_extend(p, 5)
+    assert errors() == 16 and places[0].tolist() == [rows] * 5 and places[1].tolist() == [-1] * 5
+    assert torch.equal(places[2:], table[2:, :1].expand(-1, 5)) and slots[2:].unique().tolist() == [3, 4, 5, 6, 7]
+    table[0, 0], refs[rows] = rows, 1
+    lens += 5
+    lens[1] = 7
+    assert torch.equal(p.table, table) and torch.equal(p.lens, lens) and torch.equal(p.refs, refs)
+    # a free page again: without the row that needs two, row 1 gets it
+    p.refs[rows], p.table[0, 0], p.lens[0] = 0, -1, 0
+    places, slots = pages_extend(p, 9, i32([1, 0]))
+    assert errors() == 16 and places.tolist() == [[rows - 1] + [rows] * 8, [-1] * 9] and slots[0].tolist() == [7, 0, 1, 2, 3, 4, 5, 6, 7]
+
+
 @pytest.mark.parametrize("bad", [-1, -7, 40, 2 ** 31 - 1])
 @pytest.mark.parametrize("max_pages", [6, 3000])
 def test_fork_of_a_row_whose_last_page_is_out_of_range(bad, max_pages):

@@ -14,7 +14,7 @@ VK_OK, VK_ERR_ARG, VK_ERR_CUDA, VK_ERR_UNSUPPORTED = 0, -1, -2, -3
 _STATUS = {VK_ERR_ARG: "bad argument", VK_ERR_CUDA: "CUDA error", VK_ERR_UNSUPPORTED: "unsupported geometry"}
 DEVERR = {1: "wait for a TMA stage timed out", 2: "wait for a free stage timed out",
           4: "wait for the tensor-core accumulator timed out", 8: "index out of range (access skipped)",
-          16: "no free cache page (row not changed)"}
+          16: "too few free cache pages (row not changed)"}
 
 p, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 

@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(ExtendArgs a, bool
     want += n;
   }
   const int got = free_pages(p, want < p.n_pages ? want : p.n_pages, a.free_list);
+  // a row that is refused keeps its places in the list, so that no later row takes a page that an earlier one lacked
   if (got < want)
     for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
       const int at = a.first[i];

@@ -21,7 +21,7 @@ enum ErrBits : uint32_t {
   ERR_WAIT_EMPTY = 1u << 1,   // producer gave up waiting for a free stage
   ERR_WAIT_ACCUM = 1u << 2,   // epilogue gave up waiting for the MMA accumulator
   ERR_BOUNDS = 1u << 3,       // an index failed its range check and the access was skipped
-  ERR_PAGES = 1u << 4,        // no free cache page was left; the row was not changed
+  ERR_PAGES = 1u << 4,        // too few free cache pages were left; the row was not changed
 };
 
 __device__ uint32_t g_error_word = 0;  // single translation unit: defined once here

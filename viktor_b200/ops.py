@@ -473,8 +473,9 @@ class KVPages:
 def pages_extend(pages: KVPages, count=1, rows=None):
     """Makes room for `count` more tokens in each of `rows` (int32 [n]; None: all): lens grows, and the tokens' places come
     back as (page, slot), int32 [n, count] each, to be used as the cache row and position of qkv_rope_cache.  Free pages
-    are taken the lowest first, in the order of the rows.  A row that is out of range, named before, full or for which
-    no page is left is not changed (place -1) and reported by check_device_errors()."""
+    are taken the lowest first, in the order of the rows.  A row that is out of range, named before, full or that needs more
+    pages than the rows before it have left is not changed (place -1) and reported by check_device_errors(); in the last
+    case later rows that need a page are not served either, even if fewer would have done (rows that need none are)."""
     ptr, n = pages._rows("rows", rows)
     _need(0 < count <= pages.max_pages * pages.page, "count must be 1 to the tokens of a row")
     page, slot = torch.empty(2, n, count, dtype=_I32, device=pages.device).unbind(0)
