@@ -198,3 +198,30 @@ def test_fork_of_a_row_whose_last_page_is_out_of_range(bad, max_pages):
     pages_fork(p, i32([0]), i32([4]))
     assert errors() == 0 and p.table[4, :2].tolist() == [0, 6] and p.lens[4] == 13
     assert torch.equal(p.k[:, 6, :5], p.k[:, 7, :5])
+
+
+# ------------------------------------------------------------------------------------------------ penalties
+@pytest.mark.parametrize("V", [7, 1000])
+def test_penalties_of_any_size(V):
+    """Repetition penalties whose inverse is no normal number: a logit over 1e-40 is not infinite as long as the quotient is a
+    number.  The inverse, the product and the result are off by half a step each, results below the normal numbers by half of
+    their step."""
+    from viktor_b200.ops import penalize_logits
+    g = torch.Generator().manual_seed(V)
+    reps = torch.tensor([2.0 ** -149, 1e-40, 1.1e-38, 2.0 ** -126, 1e-37, 0.5, 1.3, 8e37, 2.0 ** 126, 1.8e38, 3.4e38, INF, 0.0])
+    B = len(reps)
+    x = torch.randn(B, V, generator=g) * torch.randint(-140, 127, (B, V), generator=g).double().exp2()
+    x = x.float()
+    history = torch.randint(0, V, (B, 2 * V), generator=g)
+    lens = torch.full((B,), 2 * V, dtype=I32)
+    got = penalize_logits(x.cuda(), history.cuda(), lens.cuda(), repetition=reps.cuda()).cpu()
+    seen = torch.zeros(B, V, dtype=torch.bool).scatter_(1, history, True)
+    d, r = x.double(), reps.double()[:, None]
+    want = torch.where(seen, torch.where(d > 0, d / r, d * r), d)
+    most = float(torch.finfo(torch.float32).max)
+    beyond = want.abs() > most * (1 + 2.0 ** -22)
+    assert torch.equal(got[beyond], torch.where(want > 0, INF, -INF)[beyond].float())
+    inside = want.abs() < most * (1 - 2.0 ** -22)
+    assert bool((torch.isnan(got) == torch.isnan(want)).all())
+    off = (got.double() - want).abs() <= 3 * 2.0 ** -24 * want.abs() + 2.0 ** -149
+    assert bool(off[inside].all()), f"{int((~off[inside]).sum())} of {int(inside.sum())} off"

@@ -98,7 +98,9 @@ __global__ void __launch_bounds__(kThreads, 5) penalize_kernel(Args a) {
     bits[i] = w;
   }
   const float rep = a.repetition ? a.repetition[b] : 1.f, pres = a.presence ? a.presence[b] : 0.f;
-  const float inv = 1.f / rep, freq = a.frequency ? a.frequency[b] : 0.f;
+  // the quotient by rep: a product with 1 / (rep 2^k), then with 2^k, k 64 or -64 where the inverse of rep is no normal number, otherwise 0
+  const float two_k = fabsf(rep) < 1.17549435e-38f ? 18446744073709551616.f : fabsf(rep) > 8.5e37f ? 5.42101086e-20f : 1.f;
+  const float inv = 1.f / (rep * two_k), freq = a.frequency ? a.frequency[b] : 0.f;
   const float* bias = a.bias ? a.bias + b * a.ld_bias : nullptr;
   if (a.history) {
     const int64_t* h = a.history + b * a.ld_history;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 5) penalize_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const uint32_t c = a.wide ? counts[at + i] : w[i / 2] >> i % 2 * 16 & 0xffffu;
-          if (c > 0) l[i] = l[i] * (l[i] > 0.f ? inv : rep) - freq * c - pres;
+          if (c > 0) l[i] = (l[i] > 0.f ? l[i] * inv * two_k : l[i] * rep) - freq * c - pres;
         }
       }
     }
