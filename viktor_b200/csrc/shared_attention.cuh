@@ -501,7 +501,7 @@ VK_DEV void tail_item(const Args& a, const Plan& pl, uint8_t* smem) {
 
 // MT: 16-row tiles of a prefix item.  WT: warps of a tail item.
 template <typename T, int D, int MT, int WT>
-__global__ void __launch_bounds__(kThreads, D == 64 && MT == 1 ? 4 : 3) split_kernel(Args a, Plan pl) {
+__global__ void __launch_bounds__(kThreads, 3) split_kernel(Args a, Plan pl) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Rows found;
   // Tails do not read what wide_kernel writes, and wide_kernel lets this one start only after its own wait for what came

@@ -25,8 +25,8 @@ static int g_pdl = 1;
 
 // Per-device record of kernels whose dynamic shared-memory limit has been raised.  The first launch of each
 // kernel on a device must happen outside stream capture (engines warm up eagerly before capturing).
-// most_shared: the SM keeps as much of its memory as shared memory as it can while the kernel runs (the default division holds
-// two CTAs of 48 KB, not four).
+// most_shared: the SM keeps as much of its memory as shared memory as it can while the kernel runs, so that as many CTAs as its
+// 228 KB hold are resident whatever ran before.
 template <typename K>
 static bool ensure_smem(K kernel, int bytes, bool most_shared = false) {
   struct Entry {
@@ -892,9 +892,11 @@ int vk_scatter_embed(void* x, const int64_t* rows, int64_t n, int64_t x_rows, co
 }  // extern "C"
 
 namespace vk {
-// Splits of an axis of `most` positions among `items` independent pieces of work: as many as fill the resident CTAs (four per
-// SM) once, chunks of `shortest` to 4096 positions.  (256 groups of 4 rows, prefixes to 2049, tails to 1100: 81 us; filling
-// them twice 83 us, four times with chunks to 1024 89 us, chunks to 512 102 us: every split's result passes through memory.)
+// Splits of an axis of `most` positions among `items` independent pieces of work: at least `ctas` pieces, chunks of `shortest` to
+// 4096 positions.  ctas is four per SM, of which three are resident (64 KB of shared memory each): the fourth evens out lengths and
+// ends, more of them cost more partial results.  Whole calls of 256 groups x 4 rows (prefixes to 2049, tails to 1100) / of 4 rows x
+// 16 heads on 131071 positions / of 37 uneven groups: two or three per SM 88 to 89 / 107 / 33.5 us, four 83 / 103 / 33.4 us, eight
+// 85 / 104 / 37 us.  (148: the SMs of a B200; the workspace has one size with and without a device.)
 static int splits_of(int most, int64_t items, int shortest, int64_t ctas) {
   if (most <= 0) return 0;
   const int64_t want = (ctas + items - 1) / items, top = (most + shortest - 1) / shortest, low = (most + 4095) / 4096;
