@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from candidates_ref import attend_bounds, attend_ref
-from test_gpu_candidates import BF, HF, I32, INF, Attend, errors, i32, pool
+from test_gpu_candidates import BF, F32, HF, I32, INF, NAN, Attend, check_penal, errors, i32, penal_inputs, pool
 
 pytestmark = pytest.mark.gpu
 
@@ -121,6 +121,67 @@ def test_attention_offsets_that_descend(heads, B, P, lo):
         assert errors() == 8 and torch.equal(got[:lo], want[:lo]) and bool((ws[n:] == 255).all())
 
 
+# groups whose rows of a KV head are more than 32 (two streams take turns), and more than 128 (two streams of rows)
+WIDE = [((40, 1, 64), 1), ((40, 1, 128), 1), ((40, 1, 64), 4), ((20, 1, 128), 9), ((80, 2, 64), 3), ((40, 2, 128), 5)]
+
+
+@pytest.mark.parametrize("heads,each", WIDE)
+@pytest.mark.parametrize("more", [0, 3])
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 127, 128, 129, 192, 193, 255, 256, 257, 511, 513])
+def test_attention_wide_prefix_lengths(heads, each, n, more):
+    """Prefixes that end before, at and behind the ends of tiles, with a cache that ends there too or has NaN behind."""
+    check_attend(Attend(n, HF if n % 2 else BF, heads, [each, each + 1], [n, n - 1], [b % 4 for b in range(2 * each + 1)], 8, S=n + more))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,each", WIDE)
+def test_attention_wide_chunks_of_many_tiles(heads, each, dtype):
+    """As many groups as there are SMs, so that a chunk is a whole prefix: every number of tiles up to 12, and odd ends."""
+    lens = [0, 1, 63, 64, 65, 705] + [5 * g % 769 for g in range(146)]
+    check_attend(Attend(40, dtype, heads, [each] * len(lens), lens, [3] * (each * len(lens)), 8))
+
+
+@pytest.mark.parametrize("heads,sizes", [((8, 2, 64), [20, 0, 11]), ((8, 2, 64), [70, 0, 40]), ((6, 3, 128), [30, 0, 40]), ((8, 1, 128), [33, 0, 40])])
+def test_attention_wide_workspace_of_any_contents(heads, sizes):
+    """What the workspace holds does not matter: prefixes, tails and rows without tokens write no values."""
+    from viktor_b200._lib import load
+    from viktor_b200.ops import shared_prefix_attention
+    B = sum(sizes)
+    a = Attend(41, BF, heads, sizes, [900, 70, 0], [b % 3 * 20 for b in range(B)], 16, pad=2)
+    n = load().vk_shared_attention_workspace_bytes(B + 2, *heads, 3, 900, a.table.shape[1] * 16)
+    want, want_lse = shared_prefix_attention(*a.args(), return_lse=True)
+    for fill in (255, 0, 127):
+        ws = torch.full((n,), fill, dtype=torch.uint8, device="cuda")
+        for _ in range(2):
+            got, lse = shared_prefix_attention(*a.args(), workspace=ws, return_lse=True)
+            assert torch.equal(got[:B], want[:B]) and torch.equal(lse[:B], want_lse[:B])
+    check_attend(a)
+
+
+@pytest.mark.parametrize("sizes", [[20, 25], [40, 50]])
+def test_attention_wide_past_31_bits(sizes):
+    """Prefix rows and pages whose offsets pass 2^31 elements."""
+    a = Attend(42, BF, (8, 2, 64), sizes, [150, 150], [20] * sum(sizes), 16)
+    S = (1 << 31) // 128 + 1000
+    k = torch.full((2, S, 2, 64), NAN, dtype=BF, device="cuda")
+    v = torch.full((2, S, 2, 64), NAN, dtype=BF, device="cuda")
+    k[:, :150], v[:, :150] = a.k, a.v
+    n = (1 << 31) // (16 * 128) + 100
+    kp = torch.full((n, 16, 2, 64), NAN, dtype=BF, device="cuda")
+    vp = torch.full((n, 16, 2, 64), NAN, dtype=BF, device="cuda")
+    m = a.kp.shape[0]
+    kp[-m:], vp[-m:] = a.kp, a.vp
+    a.table = torch.where(a.table < m, a.table + (n - m), a.table)
+    a.k, a.v, a.kp, a.vp = k, v, kp, vp
+    check_attend(a)
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (6, 3, 128)])
+def test_attention_one_large_group_among_many(heads):
+    """The mean of the rows of a group chooses the kernel: here the large group goes through the one for few rows."""
+    check_attend(Attend(43, BF, heads, [1] * 40 + [300] + [1] * 160, [70 + g for g in range(201)], [b % 5 for b in range(500)], 16))
+
+
 # ------------------------------------------------------------------------------------------------ pages
 def test_extend_rows_near_31_bits():
     """A row of almost 2^31 tokens: `count` more than it has room for are refused, as many as it has room for are placed."""
@@ -225,3 +286,24 @@ def test_penalties_of_any_size(V):
     assert bool((torch.isnan(got) == torch.isnan(want)).all())
     off = (got.double() - want).abs() <= 3 * 2.0 ** -24 * want.abs() + 2.0 ** -149
     assert bool(off[inside].all()), f"{int((~off[inside]).sum())} of {int(inside.sum())} off"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, HF])
+@pytest.mark.parametrize("B,V,T,wide", [(3, 7, 20, 16), (5, 343, 1100, 352), (33, 343, 40, 352), (2, 50021, 4097, 50048), (1, 131071, 513, 131080),
+                                        (9, 16385, 70, 16400), (2, 33000, 70000, 33024)])
+def test_penalties_on_logits_of_a_wider_head(dtype, B, V, T, wide):
+    """The first V columns of rows that are padded: rows of logits and of out lie differently relative to 16 bytes, in several
+    slices and steps.  The arithmetic is the same, so the bits are those of contiguous logits; what lies between rows stays."""
+    from viktor_b200.ops import penalize_logits
+    a = penal_inputs(B, V, T, dtype, V + B)
+    want = check_penal(a).cuda()
+    rest = {k: v.cuda() for k, v in a.items() if k != "logits"}
+    rows = torch.full((B, wide), NAN, dtype=dtype, device="cuda")
+    rows[:, :V] = a["logits"].cuda()
+    got = penalize_logits(rows[:, :V], **rest)
+    assert got.is_contiguous() and torch.equal(got, want)
+    out = torch.full((B, wide + 1), 9.0, dtype=dtype, device="cuda")
+    penalize_logits(a["logits"].cuda(), out=out[:, 1:V + 1], **rest)
+    assert torch.equal(out[:, 1:V + 1], want) and bool((out[:, 0] == 9).all()) and bool((out[:, V + 1:] == 9).all())
+    penalize_logits(rows[:, :V], out=rows[:, :V], **rest)
+    assert torch.equal(rows[:, :V], want) and bool(torch.isnan(rows[:, V:]).all())
