@@ -299,8 +299,9 @@ int vk_shared_attention(const void* q, int64_t stride_q, int dtype, const void* 
 /* Pages of a cache.  table [rows, max_pages] i32 names the pages of each row (-1 behind its last), lens [rows] i32 the
  * tokens of each row, refs [n_pages] i32 how many rows name a page (0: free); page = tokens per page, a power of two,
  * 8..256.  All but the last page of a row are full and only full pages are shared.  Free pages are given out the lowest
- * first, in the order of the list.  Row numbers out of range, and all but the first naming of a row that a list names
- * twice, are skipped and reported (VK_DEVERR_BOUNDS); a row that needs more pages than the ones before it in the list
+ * first, in the order of the list.  Row numbers out of range, all but the first naming of a row that a list names twice,
+ * and rows to be extended or copied whose length or partly filled last page is out of range are skipped and reported
+ * (VK_DEVERR_BOUNDS); a row that needs more pages than the ones before it in the list
  * have left is not changed and reported (VK_DEVERR_PAGES), and so is every later row of the call that needs a page, even
  * if fewer would have done: no row takes a page that an earlier one lacked.  Calls on the same pages follow one another on one stream.
  * Workspace bytes the three calls below need for n listed rows (contents do not matter). */
@@ -314,8 +315,7 @@ int vk_pages_extend(int32_t* table, int32_t* lens, int32_t* refs, int rows, int 
 
 /* Rows dst[i] become copies of rows src[i] as they were before the call, i < n: full pages are shared, a partly filled
  * last page is copied in all layers (k, v [layers, n_pages, page, token_bytes], token_bytes a multiple of 16).  What a
- * dst row held before is released; a page released by a call is given out from the next call on.  Where the page to be
- * copied is out of range, the dst row is not changed and that is reported (VK_DEVERR_BOUNDS). */
+ * dst row held before is released; a page released by a call is given out from the next call on. */
 int vk_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int rows, int max_pages, int n_pages, int page,
                   const int32_t* src, const int32_t* dst, int n, void* k, void* v, int layers, int token_bytes,
                   void* workspace, size_t workspace_bytes, void* stream);

@@ -261,6 +261,26 @@ def test_fork_of_a_row_whose_last_page_is_out_of_range(bad, max_pages):
     assert torch.equal(p.k[:, 6, :5], p.k[:, 7, :5])
 
 
+@pytest.mark.parametrize("lens,last", [(-1, 1), (-(2 ** 31), 1), (6 * 8 + 1, 1), (2 ** 31 - 1, 1), (13, -1), (13, 40)])
+def test_extend_and_fork_of_a_row_out_of_range(lens, last):
+    """A row whose length or partly filled last page is out of range is left as it is and reported; the others are served."""
+    from viktor_b200.ops import pages_extend, pages_fork
+    p = pool()
+    pages_extend(p, 13, i32([0, 1, 2]))
+    p.lens[0], p.table[0, 1] = lens, last
+    table, lengths, refs = p.table.clone(), p.lens.clone(), p.refs.clone()
+    places, slots = pages_extend(p, 4, i32([0, 1]))
+    assert errors() == 8 and places.tolist() == [[-1] * 4, [3, 3, 3, 6]] and slots.tolist() == [[-1] * 4, [5, 6, 7, 0]]
+    table[1, 2], lengths[1], refs[6] = 6, 17, 1
+    assert torch.equal(p.table, table) and torch.equal(p.lens, lengths) and torch.equal(p.refs, refs)
+    pages_fork(p, i32([0, 2]), i32([3, 4]))
+    assert errors() == 8
+    table[4, :2], lengths[4], refs[4], refs[7] = i32([4, 7]), 13, 2, 1
+    assert torch.equal(p.table, table) and torch.equal(p.lens, lengths) and torch.equal(p.refs, refs)
+    pages_fork(p, i32([2]), i32([0]))  # over the damaged row: well again
+    assert errors() == 0 and p.lens[0] == 13
+
+
 # ------------------------------------------------------------------------------------------------ penalties
 @pytest.mark.parametrize("V", [7, 1000])
 def test_penalties_of_any_size(V):

@@ -92,11 +92,13 @@ VK_DEV void claim_rows(const int32_t* list, int n, int rows, int32_t* claim) {
   __syncthreads();
 }
 
+// The tokens of a row, -1 where its length or its partly filled last page is out of range.
 VK_DEV int row_len(const Pool& p, int row) {
-  const int len = p.lens[row], most = p.max_pages << p.page_shift;
-  if (len >= 0 && len <= most) return len;
-  raise_error(ERR_BOUNDS);
-  return len < 0 ? 0 : most;
+  const int len = p.lens[row];
+  if (len < 0 || len > p.max_pages << p.page_shift) return -1;
+  if ((len & ((1 << p.page_shift) - 1)) == 0) return len;
+  const int last = p.table[static_cast<int64_t>(row) * p.max_pages + (len >> p.page_shift)];
+  return last >= 0 && last < p.n_pages ? len : -1;
 }
 // Of a length a row can have: at most max_pages whole pages, so the sum stays below 2^31.
 VK_DEV int pages_of(const Pool& p, int len) { return (len + (1 << p.page_shift) - 1) >> p.page_shift; }
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(ExtendArgs a, bool
       if (ok) {
         const int len = row_len(p, row);
         a.len[i] = len;
-        ok = a.count <= (p.max_pages << p.page_shift) - len;  // (their sum may pass 2^31)
+        ok = len >= 0 && a.count <= (p.max_pages << p.page_shift) - len;  // (their sum may pass 2^31)
         if (ok) need = pages_of(p, len + a.count) - pages_of(p, len);
       }
       if (!ok) raise_error(ERR_BOUNDS);
@@ -258,19 +260,12 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(ForkArgs a, bool cel
     if (ok) {
       const int s = a.src[i], t = a.dst[i];
       ok = s >= 0 && s < p.rows && t >= 0 && t < p.rows && a.claim[t] == i;
-      if (!ok) raise_error(ERR_BOUNDS);
-      if (ok && s == t) ok = false;
+      const int len = ok ? row_len(p, s) : -1;
+      if (len < 0) raise_error(ERR_BOUNDS);
+      ok = len >= 0 && s != t;
       if (ok) {
-        const int len = row_len(p, s);
         a.len[i] = len;
-        if (len & mask) {  // the page to be copied
-          const int from = p.table[static_cast<int64_t>(s) * p.max_pages + (len >> p.page_shift)];
-          ok = from >= 0 && from < p.n_pages;
-          if (ok)
-            need = 1;
-          else
-            raise_error(ERR_BOUNDS);
-        }
+        need = (len & mask) != 0;
       }
     }
     int n;

@@ -473,8 +473,8 @@ class KVPages:
 def pages_extend(pages: KVPages, count=1, rows=None):
     """Makes room for `count` more tokens in each of `rows` (int32 [n]; None: all): lens grows, and the tokens' places come
     back as (page, slot), int32 [n, count] each, to be used as the cache row and position of qkv_rope_cache.  Free pages
-    are taken the lowest first, in the order of the rows.  A row that is out of range, named before, full or that needs more
-    pages than the rows before it have left is not changed (place -1) and reported by check_device_errors(); in the last
+    are taken the lowest first, in the order of the rows.  A row that is out of range, named before, full, whose length or
+    last page is out of range, or that needs more pages than the rows before it have left is not changed (place -1) and reported by check_device_errors(); in the last
     case later rows that need a page are not served either, even if fewer would have done (rows that need none are)."""
     ptr, n = pages._rows("rows", rows)
     _need(0 < count <= pages.max_pages * pages.page, "count must be 1 to the tokens of a row")
@@ -489,8 +489,8 @@ def pages_extend(pages: KVPages, count=1, rows=None):
 def pages_fork(pages: KVPages, src, dst):
     """Rows dst[i] (int32 [n]) become copies of rows src[i] as they were before the call.  Full pages are shared; a partly
     filled last page is copied in every layer.  What the dst rows held is released, and given out again from the next
-    call on.  src[i] == dst[i] leaves the row as it is.  A row that is out of range, a dst named before, or a src whose page to be
-    copied is out of range or for which no page is left changes nothing and is reported by check_device_errors()."""
+    call on.  src[i] == dst[i] leaves the row as it is.  A row that is out of range, a dst named before, or a src whose length or
+    page to be copied is out of range or for which no page is left changes nothing and is reported by check_device_errors()."""
     src_ptr, n = pages._rows("src", src)
     dst_ptr, m = pages._rows("dst", dst)
     _need(src is not None and dst is not None and n == m, "src and dst must have one length")
