@@ -325,7 +325,8 @@ int vk_pages_free(int32_t* table, int32_t* lens, int32_t* refs, int rows, int ma
                   const int32_t* list, int n, void* stream);
 
 /* Moves pages in use until they are the lowest ones: with L = the pages in use (written to live [1] i32), those
- * numbered L and above go into the free pages below L, both in ascending order; table and refs follow. */
+ * numbered L and above go into the free pages below L, both in ascending order; table and refs follow.  An entry of the
+ * table that names a free page from L on is left and reported (VK_DEVERR_BOUNDS). */
 int vk_pages_compact(int32_t* table, int32_t* refs, int rows, int max_pages, int n_pages, int page, void* k, void* v,
                      int layers, int token_bytes, int32_t* live, void* workspace, size_t workspace_bytes, void* stream);
 

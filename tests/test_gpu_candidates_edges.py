@@ -281,6 +281,22 @@ def test_extend_and_fork_of_a_row_out_of_range(lens, last):
     assert errors() == 0 and p.lens[0] == 13
 
 
+def test_compact_with_a_table_that_names_a_free_page():
+    """Such an entry is left as it is and reported, whatever the workspace held; the others follow their pages."""
+    from viktor_b200.ops import pages_compact, pages_extend, pages_free
+    p = pool(n_pages=400)
+    pages_extend(p, 13, i32([0, 1, 2]))
+    pages_free(p, i32([0]))
+    p.table[5, :3] = i32([399, 7, 401])
+    for _ in range(3):
+        filled = [torch.full((1 << k,), 5, dtype=I32, device="cuda") for k in (9, 10, 11, 12)]
+        del filled
+        p.table[2, :2], p.refs[:6] = i32([4, 5]), i32([0, 0, 1, 1, 1, 1])
+        assert int(pages_compact(p)) == 4 and errors() == 8
+        assert p.table[1, :2].tolist() == [2, 3] and p.table[2, :2].tolist() == [0, 1] and p.table[5, :3].tolist() == [399, 7, 401]
+        assert p.refs.nonzero().flatten().tolist() == [0, 1, 2, 3]
+
+
 # ------------------------------------------------------------------------------------------------ penalties
 @pytest.mark.parametrize("V", [7, 1000])
 def test_penalties_of_any_size(V):

@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(256) free_kernel(Pool p, const int32_t* list, 
 struct CompactArgs {
   Pool p;
   int32_t* holes;   // [n_pages] scratch
-  int32_t* goes;    // [n_pages] scratch: where a moved page goes
+  int32_t* goes;    // [n_pages] scratch, from number `live` on: where a moved page goes, -1: it was free
   Move* moves;      // [n_pages / 2] out
   int32_t* counts;  // [2] out: moves, pages in use
   int32_t* live;    // [1] out: pages in use
@@ -336,6 +336,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(CompactArgs a) {
   pdl_launch_dependents();
   const int live = scan_pages(p.refs, 0, p.n_pages, true, p.n_pages, [](int, int) {});
   scan_pages(p.refs, 0, live, false, live, [&](int at, int i) { a.holes[at] = i; });
+  for (int i = live + threadIdx.x; i < p.n_pages; i += kPlanThreads) a.goes[i] = -1;
+  __syncthreads();
   const int moved = scan_pages(p.refs, live, p.n_pages, true, p.n_pages, [&](int at, int i) {
     const int to = a.holes[at];
     a.moves[at] = Move{i, to, 1 << p.page_shift};
@@ -377,7 +379,12 @@ struct Renumber {
     const uint32_t cells = static_cast<uint32_t>(p.rows) * p.max_pages;  // below 2^31
     for (uint32_t x = x0; x < cells; x += step) {
       const int old = p.table[x];
-      if (old >= from && old < p.n_pages) p.table[x] = goes[old];
+      if (old < from || old >= p.n_pages) continue;
+      const int to = goes[old];
+      if (to >= 0)
+        p.table[x] = to;
+      else
+        raise_error(ERR_BOUNDS);  // the table names a page that refs holds for free
     }
   }
 };
