@@ -8,9 +8,13 @@
 // Prefix and tails are split over CTAs, each with a running maximum and sum (base 2); a last kernel joins the partial results,
 // in a fixed order, so equal calls give equal bits and nothing in the workspace outlives a call.
 //  * few rows of a group and KV head (up to 32 of D 64, 16 of D 128 on average), and every tail: split_kernel, on the warp tensor
-//    cores, bound by HBM.  256 groups of 4 rows, prefixes to 2049, tails to 1100 (451 MB): 75 us, 6.0 TB/s.  4 rows x 16 heads
-//    on 131071 positions (537 MB): 88 us, 6.1 TB/s.
+//    cores, bound by HBM.  256 groups of 4 rows, prefixes to 2049, tails to 1100 (451 MB): 77 us, 5.9 TB/s.  4 rows x 16 heads
+//    on 131071 positions (537 MB): 91 us, 5.9 TB/s.
 //  * more rows: wide_kernel, on the 5th-generation tensor cores, bound by the exponentials and the steps around them.
+// The mean is what the host knows.  Whole calls in bf16 on prefixes of 2049, split_kernel / wide_kernel: 256 groups of 4 rows x 8
+// heads on 2 of D 64 (16 rows) 77 / 112 us, of 8 rows (32) 85 / 107, of 9 rows (36) 99 / 107, of 16 rows (64) 107 / 120; 128
+// groups of 16 rows 69 / 67 us, 32 groups of 32 rows (128) 50 / 44 us; D 128, 256 groups of 4 rows (16) 128 / 159 us.  One group of
+// 256 rows among 200 of one: 62 / 83 us.
 #pragma once
 
 #include <type_traits>
@@ -505,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, 3) split_kernel(Args a, Plan pl) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Rows found;
   // Tails do not read what wide_kernel writes, and wide_kernel lets this one start only after its own wait for what came
-  // before: so behind it the tails run at once, and the wait comes last, for the kernel that joins both.
+  // before: so behind it the tails need not wait.  The wait comes last, for the kernel that joins both, and in every CTA: one that is
+  // done keeps its place until the prefix is, so that only as many tails run beside it as find a place at first.
   if (!pl.behind_wide) pdl_wait();
   pdl_launch_dependents();
   if (static_cast<int>(blockIdx.x) < pl.prefix_items) {
@@ -537,7 +542,8 @@ __global__ void __launch_bounds__(kThreads, 3) split_kernel(Args a, Plan pl) {
 // A batch of MMAs takes some 600 cycles more from issue to completion than its work (256 cycles), so nothing a stream's softmax
 // waits for may hang on its last result: the scores of tile c + 1 are issued as soon as those of c are in registers, and P
 // has a place of its own, twice.  A tile takes some 1700 cycles, the exponentials of both streams (768 of them on their pipe)
-// and the steps around them; its MMAs take 1024.  256 rows of 32 heads on 32768 positions, D 128, fp16: 147 us, 940 TFLOP/s.
+// and the steps around them; its MMAs take 1024.  256 rows of 32 heads on 32768 positions, D 128, fp16: 148 to 156 us on several cards, some
+// 900 TFLOP/s.
 // (P over the scores, in two buffers, which hung on the last result: 5 % more; one buffer of 128 positions and MMAs issued behind a
 // branch on the lane: 181 us.)
 template <int D>
@@ -825,7 +831,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float2 t = __ffma2_rn(make_float2(v[c0 + i], v[c0 + i + 1]), sc2, nm2);
-          const bool poly = i % 8 == 2;  // every fourth pair (none: 160 us, every fourth 153 us, every other one 164 us)
+          const bool poly = i % 8 == 2;  // every fourth pair (the call above with its tails: none 217 us, every fourth 215, every other one 224)
           const float2 p = poly ? poly_exp2(t) : make_float2(fast_exp2(t.x), fast_exp2(t.y));
           rs4[(i >> 1) & 3] = __fadd2_rn(rs4[(i >> 1) & 3], p);
           pk[i / 2] = pack2<T>(p.x, p.y);
